@@ -4,8 +4,11 @@ launches on the current stream and raises instead of returning a wrong result:
 refuses.  There is no CPU path: a tensor that is not on a GPU is an error."""
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
+import itertools
+import math
 import operator
 import os
 from typing import Optional
@@ -432,6 +435,93 @@ def sample(logits: torch.Tensor, temperature: Optional[torch.Tensor],
     _check(_lib("sampling").tokb200_sample(
         _ptr(logits), _i(logits.shape[0]), _i(logits.shape[1]), _ptr(temperature), _ptr(top_p),
         _ptr(uniform), _ptr(out), _stream()), "sample")
+
+
+def _here(what: str, *tensors) -> None:
+    """The tensors lie on the device whose stream the launch goes to."""
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise KernelError("tokenizer_b200 kernels run on a GPU only; got a CPU tensor")
+        device = torch.cuda.current_device()
+        if t.device.index != device:
+            raise ValueError(f"{what}: a tensor of device {t.device.index} while device {device} is the current one")
+
+
+def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: Optional[torch.Tensor], top_p: Optional[torch.Tensor],
+                    min_p: Optional[torch.Tensor], uniform: torch.Tensor, out: torch.Tensor) -> None:
+    """One token per row of float32 logits [rows, vocab], drawn behind filters.  Candidates are ordered by logit descending
+    (equal logits by id), with weights exp((l - max) / T).  Of that order are kept the first `top_k` (int32; 0 or less: all),
+    the shortest prefix whose share of what top-k left reaches `top_p` (float32; at least one; 1 or more: all) and the weights
+    of at least `min_p` times the largest (float32; 0: all; above 1 counts as 1), the shortest of the three; the draw is the
+    first candidate whose running sum passes `uniform` (float32, from [0, 1)) times the kept sum.  temperature 0 (or below, or
+    NaN) is the greedy choice, and so is a row that holds a NaN (never chosen) or a positive infinity; an id of weight 0 is
+    never drawn.  `top_k`, `top_p` and `min_p` may be None (off); each of the others has one value a row.  A row's answer
+    depends on nothing but its own logits and settings."""
+    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.shape[1] == 0:
+        raise ValueError("sample_filtered: logits are float32 [rows, vocab], with at least one id")
+    rows = logits.shape[0]
+    for t, dtype, name in ((temperature, torch.float32, "temperature"), (top_k, torch.int32, "top_k"), (top_p, torch.float32, "top_p"),
+                           (min_p, torch.float32, "min_p"), (uniform, torch.float32, "uniform"), (out, torch.int32, "out")):
+        if t is None and name in ("top_k", "top_p", "min_p"):
+            continue
+        if t is None or t.dtype != dtype or t.dim() != 1 or t.shape[0] != rows:
+            raise ValueError(f"sample_filtered: {name} is {str(dtype)[6:]}, one value for each of the {rows} rows")
+    _here("sample_filtered", logits, temperature, top_k, top_p, min_p, uniform, out)
+    _check(_lib("sample_filtered").tokb200_sample_filtered(
+        _ptr(logits), _i(rows), _i(logits.shape[1]), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(uniform),
+        _ptr(out), _stream()), "sample_filtered")
+
+
+def _flat_pairs(pairs):
+    """(source, destination, rows) triples as one array of 32-bit integers."""
+    try:
+        flat = array.array("i", itertools.chain.from_iterable(pairs))
+        whole = all(len(p) == 3 for p in pairs)
+    except (TypeError, OverflowError):
+        whole = False
+    if not whole:
+        raise ValueError("copy_pages: pairs are (source page, destination page, rows), whole numbers of 32 bits")
+    return flat
+
+
+def copy_pages(pool: torch.Tensor, page_size: int, pairs) -> None:
+    """Copies pages inside a pool [planes ..., pages * page_size, kv heads, head size] of any type, the same in every plane:
+    of each (source page, destination page, rows) in `pairs` (on the host) the first `rows` rows.  The copies have no order,
+    so no page is a destination twice, or a destination and a source."""
+    if pool.dim() < 4 or page_size < 1 or pool.shape[-3] % page_size:
+        raise ValueError("copy_pages: the pool is [planes ..., pages * page_size, kv heads, head size]")
+    pairs = list(pairs)
+    flat = _flat_pairs(pairs)
+    pages = pool.shape[-3] // page_size
+    row_bytes = pool.shape[-1] * pool.shape[-2] * pool.element_size()
+    _here("copy_pages", pool)
+    at = _ptr(pool)
+    if not pairs:
+        return
+    status = _lib("pages").tokb200_copy_pages(
+        at, _i(math.prod(pool.shape[:-3])), _ll(pages), _i(page_size), _ll(row_bytes), ctypes.c_void_p(flat.buffer_info()[0]),
+        _i(len(pairs)), _stream())
+    if status == -1:
+        _explain_pairs(pairs, pages, page_size)
+    _check(status, "copy_pages")
+
+
+def _explain_pairs(pairs, pages: int, page_size: int) -> None:
+    """Raise for the first pair that the kernel's launcher refuses."""
+    targets = set()
+    for source, target, rows in pairs:
+        if not (0 <= source < pages and 0 <= target < pages):
+            raise ValueError(f"copy_pages: page {source} or {target} is not one of the pool's {pages}")
+        if not 0 <= rows <= page_size:
+            raise ValueError(f"copy_pages: {rows} rows of a page of {page_size}")
+        if target in targets:
+            raise ValueError(f"copy_pages: page {target} is a destination twice")
+        targets.add(target)
+    for source, _, _ in pairs:
+        if source in targets:
+            raise ValueError(f"copy_pages: page {source} is a source and a destination")
 
 
 def prefetch_l2(t: torch.Tensor) -> None:

@@ -12,6 +12,8 @@ def all_variants():
         ("gemm_f32.cu", (), ()),
         ("gemm_f32_tcgen05.cu", (), ()),
         ("sampling.cu", (), ()),
+        ("sample_filtered.cu", (), ()),
+        ("pages.cu", (), ()),
         ("linear_small_m.cu", (), ()),
         ("gemm_tcgen05.cu", (), ()),
         ("ffn_small_m.cu", (), ()),
