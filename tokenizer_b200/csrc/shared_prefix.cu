@@ -1,0 +1,253 @@
+// Attention of decoding rows whose caches begin with the same pages: the general kernels (any type, head size to 256 and
+// page size; the tensor-core ones for bfloat16 are in shared_prefix_tcgen05.cu).
+//
+// A row r sees the `keys` keys of its tile, read through the table of the tile's first member, and its own keys from
+// shared[r] up to pos[r]; a row of no tile has shared[r] = 0 and sees its own alone.  With scores s = q.k * scale (capped:
+// cap * tanh(s / cap)) the output is sum(exp(s) v) / (sum(exp(s)) + exp(sink)).  A softmax splits along its keys: a part with
+// maximum m, sum l = sum(exp(s - m)) and weighted values a = sum(exp(s - m) v) joins others by sum(exp(m - M) a) / sum(exp(m -
+// M) l), M the largest m.  So the common keys are read once a tile, for all heads of all members together, the own keys once a
+// row, each cut into pieces over blocks; every piece leaves (a, m, l) in 32 bits, and a second kernel joins them.
+//
+// A block takes 32 (row, head) pairs, four a warp, and walks its piece 32 keys at a time: keys and values lie in shared
+// memory in 32 bits; a lane has a key for the scores (of its warp's four pairs at once, 16 multiply-adds for five 16-byte
+// reads of shared memory) and every 32nd lane of the head for the weighted values.
+#include "common.cuh"
+
+#define SP_WARPS 8
+#define SP_THREADS (SP_WARPS * 32)
+#define SP_PAIRS_WARP 4
+#define SP_PAIRS (SP_WARPS * SP_PAIRS_WARP)       // (row, head) pairs of a block
+#define SP_KEYS 32
+#define SP_MIN_PIECE 64
+#define SP_LOG2E 1.4426950408889634f
+
+// keys of a piece when n keys are cut into at most `pieces`
+__host__ __device__ __forceinline__ int sp_piece(int n, int pieces) {
+  const int len = ((n + pieces - 1) / pieces + SP_KEYS - 1) / SP_KEYS * SP_KEYS;
+  return len < SP_MIN_PIECE ? SP_MIN_PIECE : len;
+}
+
+// parts: [row][head][tile_pieces + own_pieces][d + 2]
+template <typename T, int DI>
+__global__ void __launch_bounds__(SP_THREADS)
+shared_prefix_parts_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, const T* __restrict__ v_pool,
+                           const int* __restrict__ block_table, int table_stride, const int* __restrict__ row_req,
+                           const int* __restrict__ pos, const int* __restrict__ shared, const int* __restrict__ members,
+                           const int4* __restrict__ tiles, int n_tiles, int nh, int nkv, int d, int page, float scale_log2,
+                           float cap_in, float cap_out, int tile_pieces, int own_pieces, float* __restrict__ parts) {
+  constexpr int kD = DI * 32, kStride = kD + 4;
+  extern __shared__ __align__(16) float sp_smem[];
+  float* q_s = sp_smem;                              // [pair][kD]
+  float* k_s = q_s + SP_PAIRS * kD;                  // [key][kStride]
+  float* v_s = k_s + SP_KEYS * kStride;              // [key][kD]
+  float4* p_s = reinterpret_cast<float4*>(v_s + SP_KEYS * kD);      // [warp][key]: the probabilities of a warp's pairs
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = nh / nkv, kvh = blockIdx.y % nkv, chunk = blockIdx.y / nkv, piece = blockIdx.x;
+  const bool common = (int)blockIdx.z < n_tiles;
+  pdl_wait();
+  pdl_launch();
+  // the block's pairs: (member, head) of a tile, or the heads of a row; its keys first..end of table `req`
+  int first_member = 0, n_pairs, req, first, end, slot;
+  const int row_alone = common ? -1 : (int)blockIdx.z - n_tiles;
+  if (common) {
+    const int4 tile = tiles[blockIdx.z];
+    const int lead = tile.y > 0 ? members[tile.x] : -1;
+    first_member = tile.x;
+    n_pairs = tile.y * group;
+    req = lead < 0 ? -1 : row_req[lead];
+    const int keys = min(tile.z, table_stride * page), len = sp_piece(keys, tile_pieces);
+    first = piece * len;
+    end = min(keys, first + len);
+    slot = piece;
+  } else {
+    n_pairs = group;
+    req = row_req[row_alone];
+    const int from = max(shared[row_alone], 0), n = min(pos[row_alone] + 1, table_stride * page) - from, len = sp_piece(max(n, 0), own_pieces);
+    first = from + piece * len;
+    end = from + min(max(n, 0), (piece + 1) * len);
+    slot = tile_pieces + piece;
+  }
+  if (req < 0 || first >= end || chunk * SP_PAIRS >= n_pairs) return;
+  auto row_of = [&](int pair) { return common ? members[first_member + pair / group] : row_alone; };
+  int row[SP_PAIRS_WARP], head[SP_PAIRS_WARP];
+#pragma unroll
+  for (int i = 0; i < SP_PAIRS_WARP; ++i) {
+    const int in_block = warp * SP_PAIRS_WARP + i, pair = chunk * SP_PAIRS + in_block;
+    row[i] = pair < n_pairs ? row_of(pair) : -1;
+    head[i] = kvh * group + pair % group;
+    const T* from = q + ((size_t)max(row[i], 0) * nh + head[i]) * d;
+#pragma unroll
+    for (int c = lane; c < kD; c += 32) q_s[in_block * kD + c] = row[i] >= 0 && c < d ? to_float(from[c]) : 0.f;
+  }
+  float m_run[SP_PAIRS_WARP], l_run[SP_PAIRS_WARP], acc[SP_PAIRS_WARP][DI];
+#pragma unroll
+  for (int i = 0; i < SP_PAIRS_WARP; ++i) {
+    m_run[i] = -INFINITY;
+    l_run[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < DI; ++c) acc[i][c] = 0.f;
+  }
+  const int* table = block_table + (size_t)req * table_stride;
+  for (int k0 = first; k0 < end; k0 += SP_KEYS) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < SP_KEYS / SP_WARPS; ++e) {
+      const int in_tile = e * SP_WARPS + warp, key = k0 + in_tile;
+      const bool on = key < end;
+      const size_t at = on ? ((size_t)max(table[key / page], 0) * page + key % page) * nkv + kvh : 0;
+#pragma unroll
+      for (int c = lane; c < kD; c += 32) {          // keys that are not seen, and lanes behind the head: zeros
+        k_s[in_tile * kStride + c] = on && c < d ? to_float(k_pool[at * d + c]) : 0.f;
+        v_s[in_tile * kD + c] = on && c < d ? to_float(v_pool[at * d + c]) : 0.f;
+      }
+    }
+    __syncthreads();
+    float s[SP_PAIRS_WARP] = {};
+    const float4* k_row = reinterpret_cast<const float4*>(k_s + lane * kStride);
+#pragma unroll 8
+    for (int c = 0; c < kD / 4; ++c) {
+      const float4 kv = k_row[c];
+#pragma unroll
+      for (int i = 0; i < SP_PAIRS_WARP; ++i) {
+        const float4 qv = reinterpret_cast<const float4*>(q_s + (warp * SP_PAIRS_WARP + i) * kD)[c];
+        s[i] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s[i]))));
+      }
+    }
+    float p[SP_PAIRS_WARP];
+#pragma unroll
+    for (int i = 0; i < SP_PAIRS_WARP; ++i) {
+      float x = cap_out > 0.f ? cap_out * tanhf(s[i] * cap_in) : s[i] * scale_log2;
+      if (k0 + lane >= end) x = -INFINITY;
+      const float m_new = fmaxf(m_run[i], warp_max(x));
+      // a part whose scores are all -inf so far has no weight yet (a NaN among them goes through)
+      const float corr = m_new == -INFINITY ? 1.f : exp2f(m_run[i] - m_new);
+      p[i] = x == -INFINITY ? 0.f : exp2f(x - m_new);
+      l_run[i] = l_run[i] * corr + warp_sum(p[i]);
+      m_run[i] = m_new;
+#pragma unroll
+      for (int c = 0; c < DI; ++c) acc[i][c] *= corr;
+    }
+    p_s[warp * SP_KEYS + lane] = make_float4(p[0], p[1], p[2], p[3]);
+    __syncwarp();
+#pragma unroll 8
+    for (int key = 0; key < SP_KEYS; ++key) {
+      const float4 pk = p_s[warp * SP_KEYS + key];
+#pragma unroll
+      for (int c = 0; c < DI; ++c) {
+        const float v = v_s[key * kD + lane + 32 * c];
+        acc[0][c] = fmaf(pk.x, v, acc[0][c]);
+        acc[1][c] = fmaf(pk.y, v, acc[1][c]);
+        acc[2][c] = fmaf(pk.z, v, acc[2][c]);
+        acc[3][c] = fmaf(pk.w, v, acc[3][c]);
+      }
+    }
+    __syncwarp();
+  }
+#pragma unroll
+  for (int i = 0; i < SP_PAIRS_WARP; ++i) {
+    if (row[i] < 0) continue;
+    float* part = parts + (((size_t)row[i] * nh + head[i]) * (tile_pieces + own_pieces) + slot) * (d + 2);
+#pragma unroll
+    for (int c = 0; c < DI; ++c)
+      if (lane + 32 * c < d) part[lane + 32 * c] = acc[i][c];
+    if (lane == 0) { part[d] = m_run[i]; part[d + 1] = l_run[i]; }
+  }
+}
+
+// a warp a (row, head)
+template <typename T>
+__global__ void __launch_bounds__(SP_THREADS)
+shared_prefix_join_kernel(const float* __restrict__ parts, const int* __restrict__ row_req, const int* __restrict__ pos,
+                          const int* __restrict__ shared, int n_rows, int nh, int d, int reach, int tile_pieces, int own_pieces,
+                          const float* __restrict__ sink, T* __restrict__ out) {
+  pdl_wait();
+  pdl_launch();
+  const int pair = blockIdx.x * SP_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (pair >= n_rows * nh) return;
+  const int row = pair / nh, head = pair % nh;
+  if (row_req[row] < 0) return;
+  const int keys = min(max(shared[row], 0), reach), n = max(min(pos[row] + 1, reach) - max(shared[row], 0), 0);
+  const int n_tile = keys > 0 ? (keys + sp_piece(keys, tile_pieces) - 1) / sp_piece(keys, tile_pieces) : 0;
+  const int n_own = n > 0 ? (n + sp_piece(n, own_pieces) - 1) / sp_piece(n, own_pieces) : 0;
+  const float* base = parts + (size_t)pair * (tile_pieces + own_pieces) * (d + 2);
+  auto part_of = [&](int i) { return base + (size_t)(i < n_tile ? i : tile_pieces + i - n_tile) * (d + 2); };
+  float m = -INFINITY;
+  for (int i = lane; i < n_tile + n_own; i += 32) m = fmaxf(m, part_of(i)[d]);
+  m = warp_max(m);
+  float den = 0.f;
+  for (int i = lane; i < n_tile + n_own; i += 32) den += exp2f(part_of(i)[d] - m) * part_of(i)[d + 1];
+  den = warp_sum(den);
+  if (sink) den += exp2f(sink[head] * SP_LOG2E - m);
+  for (int c = lane; c < d; c += 32) {
+    float num = 0.f;
+    for (int i = 0; i < n_tile + n_own; ++i) num += exp2f(part_of(i)[d] - m) * part_of(i)[c];
+    out[(size_t)pair * d + c] = from_float<T>(n_tile + n_own ? num / den : 0.f);      // a row without a key: zeros
+  }
+}
+
+// (pieces of a tile's keys, pieces of a row's own keys) for a launch of these sizes: enough blocks for the device, at most 16
+TOKB200_API int tokb200_shared_prefix_pieces(int n_rows, int n_tiles, int nkv, int reach, int* tile_pieces, int* own_pieces) {
+  const int most = (reach + SP_MIN_PIECE - 1) / SP_MIN_PIECE, blocks = 148 * 4;
+  auto cut = [&](int units) {
+    int n = units > 0 ? (blocks + units - 1) / units : 1;
+    n = n > 16 ? 16 : n;
+    return n > most ? most : n < 1 ? 1 : n;
+  };
+  *tile_pieces = cut(n_tiles * nkv);
+  *own_pieces = cut(n_rows * nkv);
+  return TOKB200_OK;
+}
+
+template <typename T, int DI>
+static int sp_launch(const void* q, const void* k_pool, const void* v_pool, void* out, const int* block_table, int table_stride,
+                     const int* row_req, const int* pos, const int* shared, const int* members, const int* tiles, int n_tiles,
+                     int tile_members, int n_rows, int nh, int nkv, int d, int page, float scale, const float* sink, float softcap,
+                     int tile_pieces, int own_pieces, float* parts, cudaStream_t stream) {
+  const int group = nh / nkv;
+  const int most_pairs = (n_tiles > 0 && tile_members > 1 ? tile_members : 1) * group;
+  const int chunks = (most_pairs + SP_PAIRS - 1) / SP_PAIRS;
+  if ((long long)nkv * chunks > 65535 || n_tiles + n_rows > 65535) return TOKB200_BAD_SIZE;
+  const size_t smem = (size_t)(SP_PAIRS * DI * 32 + SP_KEYS * (DI * 32 + 4) + SP_KEYS * DI * 32 + SP_WARPS * SP_KEYS * 4) * 4;
+  static bool configured[64] = {};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return TOKB200_BAD_SIZE;
+  if (smem > 48 * 1024 && !configured[device]) {
+    cudaError_t err = cudaFuncSetAttribute(shared_prefix_parts_kernel<T, DI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (err != cudaSuccess) return (int)err;
+    configured[device] = true;
+  }
+  const dim3 grid(tile_pieces > own_pieces ? tile_pieces : own_pieces, nkv * chunks, n_tiles + n_rows);
+  int status = launch_dependent(shared_prefix_parts_kernel<T, DI>, grid, dim3(SP_THREADS), smem, stream, (const T*)q, (const T*)k_pool,
+                                (const T*)v_pool, block_table, table_stride, row_req, pos, shared, members, (const int4*)tiles, n_tiles, nh,
+                                nkv, d, page, scale * SP_LOG2E, softcap > 0.f ? scale / softcap : 0.f,
+                                softcap > 0.f ? softcap * SP_LOG2E : 0.f, tile_pieces, own_pieces, parts);
+  if (status != TOKB200_OK) return status;
+  return launch_dependent(shared_prefix_join_kernel<T>, dim3((unsigned)((n_rows * nh + SP_WARPS - 1) / SP_WARPS)), dim3(SP_THREADS), 0, stream,
+                          parts, row_req, pos, shared, n_rows, nh, d, table_stride * page, tile_pieces, own_pieces, sink, (T*)out);
+}
+
+// tiles: [n_tiles][4] = (first place in `members`, members, keys, 0); at most `tile_members` members each.
+TOKB200_API int tokb200_shared_prefix_attention(
+    const void* q, const void* k_pool, const void* v_pool, void* out, int dtype, const int* block_table, int table_stride,
+    const int* row_req, const int* pos, const int* shared, const int* members, const int* tiles, int n_tiles, int tile_members,
+    int n_rows, int nh, int nkv, int d, int page, float scale, const float* sink, float softcap, int tile_pieces, int own_pieces,
+    float* parts, cudaStream_t stream) {
+  if (n_rows <= 0) return TOKB200_OK;
+  if (nh <= 0 || nkv <= 0 || nh % nkv || d <= 0 || d > 256 || page <= 0 || n_tiles < 0 || tile_members < 0 || tile_pieces < 1 || own_pieces < 1 ||
+      tile_pieces > 65535 || table_stride <= 0 || (long long)table_stride * page > 0x7fffffffLL || (long long)n_rows * nh > 0x7fffffffLL)
+    return TOKB200_BAD_SIZE;
+  if ((uintptr_t)tiles & 15) return TOKB200_BAD_ALIGNMENT;
+#define SP_CASE(T, DI)                                                                                                             \
+  return sp_launch<T, DI>(q, k_pool, v_pool, out, block_table, table_stride, row_req, pos, shared, members, tiles, n_tiles, tile_members, \
+                          n_rows, nh, nkv, d, page, scale, sink, softcap, tile_pieces, own_pieces, parts, stream)
+#define SP_TYPE(T)                                                                                                                 \
+  do {                                                                                                                             \
+    if (d <= 32) SP_CASE(T, 1);                                                                                                    \
+    if (d <= 64) SP_CASE(T, 2);                                                                                                    \
+    if (d <= 128) SP_CASE(T, 4);                                                                                                   \
+    SP_CASE(T, 8);                                                                                                                 \
+  } while (0)
+  if (dtype == TOKB200_F32) SP_TYPE(float);
+  if (dtype == TOKB200_BF16) SP_TYPE(__nv_bfloat16);
+  return TOKB200_BAD_DTYPE;
+}

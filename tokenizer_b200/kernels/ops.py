@@ -584,6 +584,61 @@ def decode_attention(q, k_pool, v_pool, out, block_table, row_req, pos, nh, nkv,
         _ptr(counters), _ptr(rows), _ptr(even), _sink(sink, nh), _f(softcap or 0.0), _stream()), "decode_attention")
 
 
+def shared_prefix_tile_members(nh: int, nkv: int) -> int:
+    """The most members of a tile of `shared_prefix_attention`: their heads of one group fill 256 rows."""
+    return max(1, 2 * (128 // (nh // nkv)))
+
+
+def shared_prefix_supported(nh: int, nkv: int, d: int) -> bool:
+    return nh % nkv == 0 and nh // nkv <= 128 and 1 <= d <= 256
+
+
+def shared_prefix_attention(q, k_pool, v_pool, out, block_table, row_req, pos, shared, members, tiles, nh, nkv, d, page, scale,
+                            sink: Optional[torch.Tensor] = None, softcap: Optional[float] = None) -> None:
+    """Attention for rows of one token each (float32 or bfloat16) of which some have the beginnings of their caches in
+    common: keys and values that several rows share are read once for all of them.
+
+    `tiles` is int32 [n, 4]: (first place in `members`, members, keys, unused) of rows that share their first `keys` keys, at most
+    `shared_prefix_tile_members` of them (a larger set is several tiles; a tile without members is skipped); `members`
+    (int32) are rows of the batch, each in one tile at most (-1: none); `shared` (int32, one a row) repeats the tile's
+    `keys`, 0 for a row of no tile.  The common keys are read through the block table of the tile's first member.  A row
+    then sees its own keys from `shared` up to its position, so `shared` is at most the position + 1; `shared_prefix_plan`
+    makes the three from block tables.  Rows of request -1 are left as they are.  `sink` and `softcap` as in the other
+    attention kernels; `block_table`, `row_req`, `pos` as theirs."""
+    rows = q.shape[0]
+    if q.dtype not in _DTYPE_TAG or k_pool.dtype != q.dtype or v_pool.dtype != q.dtype or out.dtype != q.dtype:
+        raise ValueError("shared_prefix_attention: q, keys, values and out are all float32 or all bfloat16")
+    if nkv < 1 or not shared_prefix_supported(nh, nkv, d):
+        raise ValueError(f"shared_prefix_attention: {nh} heads over {nkv} groups of size {d} is not taken")
+    if q.numel() != rows * nh * d or out.shape != q.shape or k_pool.shape != v_pool.shape or k_pool.numel() % (nkv * d):
+        raise ValueError("shared_prefix_attention: q and out are [rows, heads * size], the pools [slots, kv heads, size]")
+    if page < 1 or block_table.dim() != 2:
+        raise ValueError("shared_prefix_attention: a block table is [requests, pages]")
+    for t, name in ((block_table, "block_table"), (row_req, "row_req"), (pos, "pos"), (shared, "shared"), (members, "members"),
+                    (tiles, "tiles")):
+        if t.dtype != torch.int32:
+            raise ValueError(f"shared_prefix_attention: {name} is int32")
+    if row_req.numel() != rows or pos.numel() != rows or shared.numel() != rows or tiles.dim() != 2 or tiles.shape[1] != 4:
+        raise ValueError("shared_prefix_attention: row_req, pos and shared have one entry a row, tiles are [n, 4]")
+    if softcap is not None and not softcap > 0:
+        raise ValueError("shared_prefix_attention: a cap on the scores is positive")
+    _here("shared_prefix_attention", q, k_pool, v_pool, out, block_table, row_req, pos, shared, members, tiles, sink)
+    if rows == 0 or block_table.shape[1] == 0:
+        return
+    lib = _lib("shared_prefix")
+    n_tiles = tiles.shape[0]
+    tile_pieces, own_pieces = ctypes.c_int(1), ctypes.c_int(1)
+    lib.tokb200_shared_prefix_pieces(_i(rows), _i(n_tiles), _i(nkv), _i(block_table.shape[1] * page), ctypes.byref(tile_pieces),
+                                     ctypes.byref(own_pieces))
+    # of this launch alone: captured graphs and streams share nothing
+    parts = torch.empty(rows * nh * (tile_pieces.value + own_pieces.value) * (d + 2), dtype=torch.float32, device=q.device)
+    _check(lib.tokb200_shared_prefix_attention(
+        _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(out), _i(_tag(q)), _ptr(block_table), _i(block_table.shape[1]), _ptr(row_req),
+        _ptr(pos), _ptr(shared), _ptr(members), _ptr(tiles), _i(n_tiles), _i(shared_prefix_tile_members(nh, nkv)), _i(rows), _i(nh),
+        _i(nkv), _i(d), _i(page), _f(scale), _sink(sink, nh), _f(softcap or 0.0), tile_pieces, own_pieces, _ptr(parts), _stream()),
+        "shared_prefix_attention")
+
+
 _stream_plans = {}
 
 

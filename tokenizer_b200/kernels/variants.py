@@ -14,6 +14,7 @@ def all_variants():
         ("sampling.cu", (), ()),
         ("sample_filtered.cu", (), ()),
         ("pages.cu", (), ()),
+        ("shared_prefix.cu", (), ()),
         ("linear_small_m.cu", (), ()),
         ("gemm_tcgen05.cu", (), ()),
         ("ffn_small_m.cu", (), ()),
