@@ -142,7 +142,7 @@ class scratch_scope:
 # loaded; the host reads the word (plain memory, no CUDA call) wherever it has just
 # synchronised with the device, and raises.
 _LIBRARY_NAMES = {1: "gemm_tcgen05", 2: "attention_tcgen05", 3: "ffn_small_m", 4: "linear_stream",
-                  5: "layer_small_m", 6: "gemm_f32_tcgen05"}
+                  5: "layer_small_m", 6: "gemm_f32_tcgen05", 7: "shared_prefix_tcgen05"}
 _REASONS = {1: "a wait on a shared-memory barrier ran out", 2: "a wait between blocks ran out"}
 _error_word = None          # (ctypes int at the host address, device address)
 _registered = {}            # id(library handle) -> handle: libraries that know the word
@@ -204,7 +204,8 @@ def raise_if_error(where: str = "") -> None:
     for lib in _registered.values():          # clear the per-library flags too
         for name in ("tokb200_gemm_tcgen05_error", "tokb200_attention_tcgen05_error",
                      "tokb200_ffn_small_m_error", "tokb200_linear_stream_error",
-                     "tokb200_layer_small_m_error", "tokb200_gemm_f32_tcgen05_error"):
+                     "tokb200_layer_small_m_error", "tokb200_gemm_f32_tcgen05_error",
+                     "tokb200_shared_prefix_tcgen05_error"):
             try:
                 getattr(lib, name)()
             except AttributeError:
@@ -593,6 +594,11 @@ def shared_prefix_supported(nh: int, nkv: int, d: int) -> bool:
     return nh % nkv == 0 and nh // nkv <= 128 and 1 <= d <= 256
 
 
+def shared_prefix_tcgen05_supported(nh: int, nkv: int, d: int, page: int) -> bool:
+    """Sizes that the tensor-core kernels take in bfloat16; others go to the general ones."""
+    return d in (64, 128) and nh % nkv == 0 and nh // nkv <= DECODE_MAX_GROUP and page % 8 == 0
+
+
 def shared_prefix_attention(q, k_pool, v_pool, out, block_table, row_req, pos, shared, members, tiles, nh, nkv, d, page, scale,
                             sink: Optional[torch.Tensor] = None, softcap: Optional[float] = None) -> None:
     """Attention for rows of one token each (float32 or bfloat16) of which some have the beginnings of their caches in
@@ -625,12 +631,24 @@ def shared_prefix_attention(q, k_pool, v_pool, out, block_table, row_req, pos, s
     _here("shared_prefix_attention", q, k_pool, v_pool, out, block_table, row_req, pos, shared, members, tiles, sink)
     if rows == 0 or block_table.shape[1] == 0:
         return
-    lib = _lib("shared_prefix")
-    n_tiles = tiles.shape[0]
+    n_tiles, reach = tiles.shape[0], block_table.shape[1] * page
     tile_pieces, own_pieces = ctypes.c_int(1), ctypes.c_int(1)
-    lib.tokb200_shared_prefix_pieces(_i(rows), _i(n_tiles), _i(nkv), _i(block_table.shape[1] * page), ctypes.byref(tile_pieces),
-                                     ctypes.byref(own_pieces))
-    # of this launch alone: captured graphs and streams share nothing
+    # the parts are of this launch alone: captured graphs and streams share nothing
+    if q.dtype == torch.bfloat16 and shared_prefix_tcgen05_supported(nh, nkv, d, page) and \
+            (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr() | out.data_ptr()) % 16 == 0:
+        lib = _load("shared_prefix_tcgen05.cu", defines=(f"HEAD_DIM={d}",))
+        lib.tokb200_shared_prefix_tcgen05_pieces(_i(rows), _i(n_tiles), _i(nkv), _i(reach), ctypes.byref(tile_pieces), ctypes.byref(own_pieces))
+        parts = rows * nh * tile_pieces.value if n_tiles else 0
+        acc = torch.empty(parts * d, dtype=torch.float32, device=q.device)
+        stat = torch.empty(parts * 2, dtype=torch.float32, device=q.device)
+        _check(lib.tokb200_shared_prefix_tcgen05(
+            _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(out), _ptr(block_table), _i(block_table.shape[1]), _ptr(row_req), _ptr(pos),
+            _ptr(shared), _ptr(members), _ptr(tiles), _i(n_tiles), _i(rows), _i(k_pool.numel() // (nkv * d)), _i(nh), _i(nkv), _i(d),
+            _i(page), _f(scale), _sink(sink, nh), _f(softcap or 0.0), tile_pieces, own_pieces, _ptr(acc), _ptr(stat), _stream()),
+            "shared_prefix_attention")
+        return
+    lib = _lib("shared_prefix")
+    lib.tokb200_shared_prefix_pieces(_i(rows), _i(n_tiles), _i(nkv), _i(reach), ctypes.byref(tile_pieces), ctypes.byref(own_pieces))
     parts = torch.empty(rows * nh * (tile_pieces.value + own_pieces.value) * (d + 2), dtype=torch.float32, device=q.device)
     _check(lib.tokb200_shared_prefix_attention(
         _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(out), _i(_tag(q)), _ptr(block_table), _i(block_table.shape[1]), _ptr(row_req),

@@ -45,5 +45,7 @@ def all_variants():
     for head_dim in (64, 128):
         jobs.append(("attention_tcgen05.cu", (f"HEAD_DIM={head_dim}",), ()))
     for head_dim in (64, 128):
+        jobs.append(("shared_prefix_tcgen05.cu", (f"HEAD_DIM={head_dim}",), ()))
+    for head_dim in (64, 128):
         jobs.append(("layer_small_m.cu", (f"HEAD_DIM={head_dim}",), ()))
     return jobs
