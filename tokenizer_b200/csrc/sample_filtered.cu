@@ -11,40 +11,39 @@
 //
 // The order is never made.  A row's logits are read once, into the shared memory of its cluster's blocks; what follows goes
 // by narrowing down:
-//   1. the largest logit, its lowest id (the greedy choice), the smallest finite one;
-//   2. how many candidates lie in each of 2,048 bins of equal width below the largest (one shared-memory count a
-//      candidate), and, unless top-k says what is summed, the sum of all weights;
-//   3. the first block adds the bins up.  A bin's weights lie between those of its edges, so the counts alone bound every
-//      running sum from both sides.  Where all that can be kept fits a list (2,048: top-k of the usual sizes, the nucleus
-//      of a confident model) it is fetched, sorted, and everything is decided there;
-//   4. else each border in turn (what top-k keeps, the nucleus, the draw): the bins that can hold it are fetched and
-//      sorted, with the exact sum of what lies in front of them; where they hold more than the list, they are first cut
-//      into 2,048 finer bins with exact sums;
-//   5. candidates that finer bins cannot tell apart (equal or almost equal logits by the thousand) are told apart by the
-//      64 bits of (logit, id) themselves, 11 bits a pass.
+//   1. the largest logit, the smallest finite one;
+//   2. how many candidates lie in each of 2,048 bins of equal width below the largest and, unless top-k keeps few, the sum of
+//      their weights (shared-memory additions, a count and a low word a candidate, now and then a high word);
+//   3. the first block adds the bins up: it knows the bin of every border (what top-k keeps, the nucleus, the draw) and the
+//      exact sum in front of it.  Where all bins that can be kept fit a list (2,048 candidates: top-k of the usual sizes, the
+//      nucleus of a confident model), they are fetched once and everything is decided there; else a border's bin is fetched
+//      at a time;
+//   4. a list of up to 256 is ranked by comparing all with all; of a longer one the place of a goal is found among 2,048 finer
+//      bins, whose few candidates are then ranked;
+//   5. bins of more than 2,048 candidates (equal or almost equal logits by the thousand) are told apart by the 64 bits of
+//      (logit, id) themselves, 11 bits a pass over the row.
 #include "common.cuh"
 
-#define FS_THREADS 512
+#define FS_THREADS 1024
 #define FS_WARPS (FS_THREADS / 32)
 #define FS_BINS 2048
 #define FS_LIST 2048
-#define FS_EACH 4                    // bins of a thread, and places of the sorted list
+#define FS_EACH 2                    // bins of a thread, and candidates of the list
+#define FS_FEW 256                   // candidates that are ranked by comparing all with all
 #define FS_MAX_CLUSTER 8
-static_assert(FS_BINS == FS_THREADS * FS_EACH && FS_LIST == FS_BINS, "a thread has four bins and four places of the list");
+static_assert(FS_BINS == FS_THREADS * FS_EACH && FS_LIST == FS_BINS, "a thread has two bins and two candidates of the list");
 
 typedef unsigned long long u64;
 
-enum : int { FS_FETCH = 1, FS_FINE = 2, FS_FETCH_FINE = 3, FS_RADIX = 4, FS_FETCH_ORDER = 5 };
+enum : int { FS_COUNTS = 1, FS_SUMS = 2, FS_RADIX = 3, FS_FETCH = 4, FS_FETCH_ORDER = 5 };
 
-// What the first block asks of the cluster: candidates of bins first..last (cut into finer bins with `fine_scale`, of which
-// it may want `fine` alone), or those whose place in the order lies in low..high (cut by `shift`).
+// What the blocks of a cluster do next: count the candidates of all bins, count them and add up their weights, cut the candidates
+// whose place in the order lies in low..high by `shift`, fetch the candidates of bins first..last into the first block's list,
+// or those whose place lies in low..high.
 struct __align__(16) FsCommand {
-  int what, first, last, fine;
+  int what, first, last, shift;
   u64 low, high;
-  int shift;
-  float fine_scale;
-  int want_front, want_m;            // the sum of what lies in front; the sum of the weights above min-p's border
-  int is_last, unused[3];            // nothing is asked behind this
+  int is_first, is_last, unused[2];  // nothing was asked in front of this, nothing is behind it
 };
 
 struct __align__(16) FsStats { float max, min; int odd, unused; };       // odd: a NaN or +infinity
@@ -59,10 +58,9 @@ __device__ __forceinline__ unsigned fs_peer(const void* local, unsigned rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(theirs) : "r"((unsigned)__cvta_generic_to_shared(local)), "r"(rank));
   return theirs;
 }
-__device__ __forceinline__ uint4 fs_load128(const void* local, unsigned rank) {
-  uint4 v;
-  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(fs_peer(local, rank)) : "memory");
+__device__ __forceinline__ uint2 fs_load64(const void* local, unsigned rank) {
+  uint2 v;
+  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(fs_peer(local, rank)));
   return v;
 }
 __device__ __forceinline__ void fs_store128(const void* local, unsigned rank, uint4 v) {
@@ -109,14 +107,17 @@ struct FsWeight {
   __device__ __forceinline__ u64 operator()(float l) const { return whole(plain(l)); }
 };
 
+// how far a range of the order is shifted to leave fewer than FS_BINS parts
+__device__ __forceinline__ int fs_shift(u64 range) { return max(0, 53 - __clzll((long long)range)); }
+
 struct FsShared {
-  u64 list[FS_LIST];                 // candidates; the sums of finer bins take the same place, low words and high words
+  u64 list[FS_LIST];                 // candidates; the sums of bins take the same place, low words and high words
   unsigned count[FS_BINS];
   FsCommand command;
   FsStats stats[FS_MAX_CLUSTER];     // of the cluster's blocks, each written by its block
   uint4 ids[FS_MAX_CLUSTER];         // the first block's: the first id with the largest logit in each block's slice (x)
-  ulonglong2 sums[FS_MAX_CLUSTER];   // the first block's: of each block all weights (or those in front), those above min-p's border
-  u64 scratch[2][3 * FS_WARPS];      // taken in turn, so that one barrier an exchange is enough
+  ulonglong2 sums[FS_MAX_CLUSTER];   // the first block's: the weights above min-p's border in each block's slice (x)
+  u64 scratch[2][2 * FS_WARPS];      // taken in turn, so that one barrier an exchange is enough
   double table[64];
   float of_warps[3][FS_WARPS];
   unsigned listed, mine;
@@ -154,74 +155,34 @@ struct FsBlock {
     __syncthreads();
     return at[0];
   }
-  // sums of the threads in front of this one, of three numbers at once
-  template <typename A, typename B, typename C>
-  __device__ __forceinline__ void before(A& a, B& b, C& c) {
+  // the count and the sum of the threads in front of this one, added to `count` and `sum`
+  __device__ __forceinline__ void before(unsigned n, u64 v, unsigned& count, u64& sum) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    u64* at = next();
-    A* at_a = reinterpret_cast<A*>(at);
-    B* at_b = reinterpret_cast<B*>(at + FS_WARPS);
-    C* at_c = reinterpret_cast<C*>(at + 2 * FS_WARPS);
-    A sa = a; B sb = b; C sc = c;
+    u64* at_v = next();
+    unsigned* at_n = reinterpret_cast<unsigned*>(at_v + FS_WARPS);
+    unsigned to_n = n;
+    u64 to_v = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const A ua = __shfl_up_sync(0xffffffffu, sa, o);
-      const B ub = __shfl_up_sync(0xffffffffu, sb, o);
-      const C uc = __shfl_up_sync(0xffffffffu, sc, o);
-      if (lane >= o) { sa += ua; sb += ub; sc += uc; }
+      const unsigned un = __shfl_up_sync(0xffffffffu, to_n, o);
+      const u64 uv = __shfl_up_sync(0xffffffffu, to_v, o);
+      if (lane >= o) { to_n += un; to_v += uv; }
     }
-    if (lane == 31) { at_a[warp] = sa; at_b[warp] = sb; at_c[warp] = sc; }
+    if (lane == 31) { at_n[warp] = to_n; at_v[warp] = to_v; }
     __syncthreads();
-    A fa = 0; B fb = 0; C fc = 0;
-    for (int w = 0; w < warp; ++w) { fa += at_a[w]; fb += at_b[w]; fc += at_c[w]; }
-    a = fa + sa - a; b = fb + sb - b; c = fc + sc - c;
+    // the warps in front: a lane each
+    unsigned front_n = lane < warp ? at_n[lane & (FS_WARPS - 1)] : 0;
+    u64 front_v = lane < warp ? at_v[lane & (FS_WARPS - 1)] : 0;
+    front_n = __reduce_add_sync(0xffffffffu, front_n);
+#pragma unroll
+    for (int o = FS_WARPS / 2; o > 0; o >>= 1) front_v += __shfl_xor_sync(0xffffffffu, front_v, o);
+    front_v = __shfl_sync(0xffffffffu, front_v, 0);
+    count += front_n + to_n - n;
+    sum += front_v + to_v - v;
   }
 };
 
-// Descending order of FS_LIST numbers (or of the first `n`, a power of two from 128 on), four to a thread side by side: a warp's
-// 128 exchange in registers, pairs further apart through `list`.
-__device__ __forceinline__ void fs_sort(u64 (&v)[FS_EACH], u64* list, int n) {
-  const int tid = threadIdx.x, base = tid * FS_EACH;
-  auto keep = [](u64& a, u64& b, bool down) { if ((a < b) == down) { const u64 x = a; a = b; b = x; } };
-  for (int k = 2; k <= n; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      if (j >= 128) {
-        __syncthreads();
-        if (base < n) {
-#pragma unroll
-          for (int i = 0; i < FS_EACH; ++i) list[base + i] = v[i];
-        }
-        __syncthreads();
-        if (base < n) {
-#pragma unroll
-          for (int i = 0; i < FS_EACH; ++i) {
-            const int at = base + i;
-            const u64 other = list[at ^ j];
-            const bool larger = ((at & k) == 0) == ((at & j) == 0);        // this place keeps the larger of the two
-            if ((other > v[i]) == larger) v[i] = other;
-          }
-        }
-      } else if (base < n) {                                              // whole warps
-        if (j >= 4) {
-#pragma unroll
-          for (int i = 0; i < FS_EACH; ++i) {
-            const u64 other = __shfl_xor_sync(0xffffffffu, v[i], j >> 2);
-            const bool larger = (((base + i) & k) == 0) == (((base + i) & j) == 0);
-            if ((other > v[i]) == larger) v[i] = other;
-          }
-        } else if (j == 2) {
-          const bool down = (base & k) == 0;                              // k >= 4: the same for a thread's four
-          keep(v[0], v[2], down);
-          keep(v[1], v[3], down);
-        } else {
-          keep(v[0], v[1], (base & k) == 0);
-          keep(v[2], v[3], ((base + 2) & k) == 0);
-        }
-      }
-    }
-}
-
-__global__ void __launch_bounds__(FS_THREADS, 2)
+__global__ void __launch_bounds__(FS_THREADS, 1)
 sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, int resident, int unit_bits,
                        const float* __restrict__ temperature, const int* __restrict__ top_k, const float* __restrict__ top_p,
                        const float* __restrict__ min_p, const float* __restrict__ uniform, int* __restrict__ out) {
@@ -248,8 +209,13 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
   };
   auto group_of = [&](int i) { return resident ? held[i] : fetch4(i); };
   auto id_of = [&](int i, int e) { return begin + 4 * i - skew + e; };
+  unsigned* low_word = reinterpret_cast<unsigned*>(sh.list);
+  unsigned* high_word = low_word + FS_BINS;
+  auto clear = [&]() {
 #pragma unroll
-  for (int i = 0; i < FS_EACH; ++i) sh.count[tid + i * FS_THREADS] = 0;
+    for (int i = 0; i < FS_EACH; ++i) sh.count[tid + i * FS_THREADS] = low_word[tid + i * FS_THREADS] = high_word[tid + i * FS_THREADS] = 0;
+  };
+  clear();
   if (tid < 64) sh.table[tid] = exp2(tid / 64.0);
   if (tid == 0) { sh.listed = 0; sh.mine = 0; sh.first_id = 0x7fffffff; }
   pdl_wait();
@@ -342,131 +308,94 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
   const bool by_m = m_asked > 0.f, by_p = p_asked < 1.f;
   const double m_border = fmin((double)m_asked, 1.0), p_share = fmax((double)p_asked, 0.0);
   FsBlock block{sh, 0};
-  auto tell = [&](u64 a, u64 b) {                                 // the first block, of this one's sums
-    fs_store128(&sh.sums[rank], 0, make_uint4((unsigned)a, (unsigned)(a >> 32), (unsigned)b, (unsigned)(b >> 32)));
+  // top-k of few: the bins' counts alone say what to fetch
+  const bool count_only = by_k && k_asked <= FS_LIST / 2;
+  auto add_to = [&](int at, u64 w) {
+    const unsigned low = (unsigned)w, old = atomicAdd(&low_word[at], low);
+    const unsigned high = (unsigned)(w >> 32) + (old + low < old);
+    if (high) atomicAdd(&high_word[at], high);
   };
-  {
-    u64 sum = 0, m_sum = 0;
+  // counts of the bins and, with `sums`, their weights and the sum of those above min-p's border (told to the first block)
+  auto add_bins = [&](bool sums) {
+    u64 m_sum = 0;
     for (int i = tid; i < groups; i += FS_THREADS) {
       const float4 v = group_of(i);
       const float x[4] = {v.x, v.y, v.z, v.w};
+      int at[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (x[c] > -INFINITY) atomicAdd(&sh.count[bin_of(place_of(x[c]))], 1u);
-      if (!by_k) {
+      for (int c = 0; c < 4; ++c) {
+        at[c] = bin_of(place_of(x[c]));
+        if (x[c] > -INFINITY) atomicAdd(&sh.count[at[c]], 1u);
+      }
+      if (sums) {
         double w[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) w[c] = weight.plain(x[c]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          sum += weight.whole(w[c]);
-          if (by_m && w[c] >= m_border) m_sum += weight.whole(w[c]);
+          const u64 whole = weight.whole(w[c]);
+          if (whole) add_to(at[c], whole);
+          if (by_m && w[c] >= m_border) m_sum += whole;
         }
       }
     }
-    if (!by_k) {
-      sum = block.sum(sum);
-      if (by_m) m_sum = block.sum(m_sum);
+    if (sums && by_m) {
+      m_sum = block.sum(m_sum);
+      if (tid == 0) fs_store128(&sh.sums[rank], 0, make_uint4((unsigned)m_sum, (unsigned)(m_sum >> 32), 0u, 0u));
     }
-    if (tid == 0) tell(sum, m_sum);
-  }
-  fs_sync();
-
-  // ---- what the first block asks for, by all blocks: candidates into its list, or counts and sums of what is cut ----
+  };
+  // ---- what the first block asks for, by all blocks ----
   auto serve = [&](const FsCommand& c) {
-    const bool cut = c.what == FS_FINE || c.what == FS_RADIX;
-    u64 front = 0, m_sum = 0;
-    unsigned* low_word = reinterpret_cast<unsigned*>(sh.list);
-    unsigned* high_word = low_word + FS_BINS;
-    if (cut) {
-      // the first block has the counts of all bins in its threads' registers by now
-#pragma unroll
-      for (int i = 0; i < FS_EACH; ++i) sh.count[tid + i * FS_THREADS] = low_word[tid + i * FS_THREADS] = high_word[tid + i * FS_THREADS] = 0;
-    }
-    if (tid == 0) sh.mine = 0;
-    __syncthreads();
-    auto take = [&](float l, int id) {
-      if (rank == 0) {
-        const unsigned to = atomicAdd(&sh.listed, 1u);
-        if (to < FS_LIST) sh.list[to] = fs_order(l, id);
-      } else {
-        const unsigned to = atomicAdd(&sh.mine, 1u);
-        if (to < FS_LIST) sh.list[to] = fs_order(l, id);
+    if (c.what <= FS_RADIX) {
+      if (!c.is_first) {                           // they are clear; the first block has what they were in its threads' registers
+        clear();
+        __syncthreads();
       }
+      if (c.what <= FS_SUMS) {
+        add_bins(c.what == FS_SUMS);
+        return;
+      }
+    } else {
+      if (tid == 0) sh.mine = 0;
+      __syncthreads();
+    }
+    auto take = [&](float l, int id) {
+      const unsigned to = atomicAdd(rank == 0 ? &sh.listed : &sh.mine, 1u);
+      if (to < FS_LIST) sh.list[to] = fs_order(l, id);
     };
     if (c.what == FS_FETCH) {
       // a place lies in bins first..last where first <= place < last + 1 (the last bin has no end: nothing is >= a NaN; a place that
       // is a NaN lies in bin 0)
-      const float low = c.first > 0 ? (float)c.first : -1.f, high = c.last < FS_BINS - 1 ? (float)(c.last + 1) : __int_as_float(0x7fc00000);
+      const float low = (float)c.first, high = c.last < FS_BINS - 1 ? (float)(c.last + 1) : __int_as_float(0x7fc00000);
+      const bool from_top = c.first == 0;
       for (int i = tid; i < groups; i += FS_THREADS) {
         const float4 v = group_of(i);
         const float x[4] = {v.x, v.y, v.z, v.w};
-        double w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float p = place_of(x[e]);
-          const bool ahead = p < low || (c.first > 0 && !(p >= 0.f));
-          if (x[e] > -INFINITY && !ahead && !(p >= high)) take(x[e], id_of(i, e));
-          w[e] = c.want_front && ahead ? 1.0 : 0.0;
-        }
-        if (c.want_front && w[0] + w[1] + w[2] + w[3] > 0.0) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) front += w[e] > 0.0 ? weight(x[e]) : 0ull;
-        }
-        if (c.want_m) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = weight.plain(x[e]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) m_sum += w[e] >= m_border ? weight.whole(w[e]) : 0ull;
+          if (x[e] > -INFINITY && (from_top || p >= low) && !(p >= high)) take(x[e], id_of(i, e));
         }
       }
     } else {
-      const bool by_order = c.what == FS_RADIX || c.what == FS_FETCH_ORDER;
       for (int i = tid; i < groups; i += FS_THREADS) {
         const float4 v = group_of(i);
 #pragma unroll 1
         for (int e = 0; e < 4; ++e) {
           const float l = e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w;
-          if (!(l > -INFINITY)) continue;
-          bool in, ahead;
-          int at;
-          if (by_order) {
-            const u64 order = fs_order(l, id_of(i, e));
-            in = order >= c.low && order <= c.high;
-            ahead = order > c.high;
-            at = (int)((c.high - order) >> c.shift);
-          } else {
-            const float x = place_of(l);
-            const int b = bin_of(x);
-            in = b >= c.first && b <= c.last;
-            ahead = b < c.first;
-            at = min(FS_BINS - 1, (int)((x - (float)c.first) * c.fine_scale));
-            if (in && !cut) {
-              ahead = at < c.fine;
-              in = at == c.fine;
-            }
-          }
-          if (in && cut) {
-            const u64 w = weight(l);
+          const u64 order = fs_order(l, id_of(i, e));
+          if (!(l > -INFINITY) || order < c.low || order > c.high) continue;
+          if (c.what == FS_RADIX) {
+            const int at = (int)((c.high - order) >> c.shift);
             atomicAdd(&sh.count[at], 1u);
-            const unsigned low = (unsigned)w, old = atomicAdd(&low_word[at], low);
-            const unsigned high = (unsigned)(w >> 32) + (old + low < old);
-            if (high) atomicAdd(&high_word[at], high);
-          } else if (in) {
+            add_to(at, weight(l));
+          } else {
             take(l, id_of(i, e));
-          }
-          if (ahead) front += weight(l);
-          if (c.want_m) {
-            const double w = weight.plain(l);
-            if (w >= m_border) m_sum += weight.whole(w);
           }
         }
       }
     }
-    if (c.want_front) front = block.sum(front);
-    if (c.want_m) m_sum = block.sum(m_sum);
-    if (tid == 0) tell(front, m_sum);
-    if (!cut && rank != 0) {
+    if (c.what != FS_RADIX && rank != 0) {
       __syncthreads();
       const unsigned mine = min(sh.mine, (unsigned)FS_LIST);
       if (mine) {                                  // the same for the block
@@ -476,18 +405,286 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
       }
     }
   };
-  if (rank != 0) {
-    while (true) {
-      fs_sync();                                 // a command is there
-      const FsCommand c = sh.command;
-      serve(c);
-      fs_sync();                                 // it has been carried out
-      if (c.is_last) return;
+  // counts and sums of the thread's bins over `blocks` blocks, then running ones, from `front` on
+  unsigned count_of[FS_EACH] = {}, count_to[FS_EACH] = {};
+  u64 sum_to[FS_EACH] = {};
+  auto add_up = [&](unsigned blocks, bool sums, unsigned n_front, u64 front, unsigned (&of)[FS_EACH], unsigned (&to)[FS_EACH], u64 (&sum)[FS_EACH]) {
+#pragma unroll
+    for (int i = 0; i < FS_EACH; ++i) { of[i] = 0; sum[i] = 0; }
+    // all loads of four blocks are asked for before the first is used (one behind the other they took 1.4 us each); a block that
+    // is not there: the first one's, which count for nothing
+#pragma unroll
+    for (unsigned r0 = 0; r0 < FS_MAX_CLUSTER; r0 += 4) {
+      if (r0 >= blocks) break;
+      uint2 n[4], a[4], b[4];
+#pragma unroll
+      for (unsigned e = 0; e < 4; ++e) n[e] = fs_load64(&sh.count[tid * FS_EACH], r0 + e < blocks ? r0 + e : 0);
+      if (sums) {
+#pragma unroll
+        for (unsigned e = 0; e < 4; ++e) {
+          a[e] = fs_load64(low_word + tid * FS_EACH, r0 + e < blocks ? r0 + e : 0);
+          b[e] = fs_load64(high_word + tid * FS_EACH, r0 + e < blocks ? r0 + e : 0);
+        }
+      }
+#pragma unroll
+      for (unsigned e = 0; e < 4; ++e) {
+        if (r0 + e < blocks) {
+          of[0] += n[e].x;
+          of[1] += n[e].y;
+          if (sums) {
+            sum[0] += a[e].x + ((u64)b[e].x << 32);
+            sum[1] += a[e].y + ((u64)b[e].y << 32);
+          }
+        }
+      }
     }
-  }
+    to[0] = of[0];
+#pragma unroll
+    for (int i = 1; i < FS_EACH; ++i) { to[i] = to[i - 1] + of[i]; sum[i] += sum[i - 1]; }
+    block.before(to[FS_EACH - 1], sum[FS_EACH - 1], n_front, front);
+#pragma unroll
+    for (int i = 0; i < FS_EACH; ++i) { to[i] += n_front; sum[i] += front; }
+  };
+  // the first of all places (a thread has FS_EACH) whose test holds; FS_BINS if none does
+  auto first_of = [&](auto holds) {
+    unsigned at = FS_BINS;
+#pragma unroll
+    for (int i = FS_EACH - 1; i >= 0; --i)
+      if (holds(i)) at = tid * FS_EACH + i;
+    return (int)block.min(at);
+  };
+  // a number that the threads have FS_EACH of, at a place
+  auto at_place = [&](const auto& v, int b) {
+    u64 mine = 0;
+#pragma unroll
+    for (int i = 0; i < FS_EACH; ++i)
+      if ((b & (FS_EACH - 1)) == i) mine = (u64)v[i];
+    return block.from(tid == b / FS_EACH, mine);
+  };
 
-  // ---- 3. the first block decides ----
-  auto ask = [&](const FsCommand& c) {
+  // A goal: the goal-th candidate of the order (by_count), or the first whose running sum is > goal (strict) or >= goal.
+  struct Goal {
+    bool by_count, strict;
+    double goal;
+    __device__ __forceinline__ bool reached(unsigned count, u64 sum) const {
+      return by_count ? (double)count >= goal : strict ? (double)sum > goal : (double)sum >= goal;
+    }
+  };
+  struct Found { u64 sum, order; };              // the running sum at the candidate, its place in the order
+
+  // ---- 4. the list: in threads' registers, with weights; behind `n_front` candidates of sum `front` ----
+  u64 order_at[FS_EACH], weight_at[FS_EACH];
+  int in_list = 0;
+  unsigned n_front = 0, rank_at = 0;
+  u64 front = 0, ranked_sum = 0, ranked = 0;     // of a list of few: this thread's candidate, its rank, the running sum there
+  // ranks of the first n candidates in sh.list, weights behind them at FS_FEW
+  auto rank_few = [&](int n, unsigned count, u64 sum) {
+    rank_at = count;
+    ranked_sum = sum;
+    ranked = tid < n ? sh.list[tid] : 0;
+    if (tid < n) {
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) {
+        const u64 other = sh.list[j], w = sh.list[FS_FEW + j];
+        if (other >= ranked) { ++rank_at; ranked_sum += w; }
+      }
+    }
+  };
+  // among n ranked ones
+  auto first_ranked = [&](int n, const Goal& goal) {
+    const unsigned at = block.min(tid < n && goal.reached(rank_at, ranked_sum) ? rank_at : 0xffffffffu);
+    const unsigned most = block.min(tid < n ? ~rank_at : 0xffffffffu);       // none reaches it: the last one
+    const bool mine = tid < n && rank_at == (at == 0xffffffffu ? ~most : at);
+    const u64 sum = block.from(mine, ranked_sum);
+    return Found{sum, block.from(mine, ranked)};
+  };
+  // a longer one: cut into 2,048 parts of its order (or of low..high of it, behind `count` candidates of sum `sum`)
+  unsigned list_of[FS_EACH], list_to[FS_EACH];
+  u64 list_sum[FS_EACH], least = 0, most = 0, cut_low = 0, cut_high = 0, cut_sum = 0;
+  int cut_shift = 0;
+  auto cut_list = [&](u64 low, u64 high, unsigned count, u64 sum) {
+    cut_low = low;
+    cut_high = high;
+    cut_sum = sum;
+    cut_shift = fs_shift(high - low);
+    __syncthreads();
+    clear();
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < FS_EACH; ++i)
+      if (tid + i * FS_THREADS < in_list && order_at[i] >= low && order_at[i] <= high) {
+        const int at = (int)((high - order_at[i]) >> cut_shift);
+        atomicAdd(&sh.count[at], 1u);
+        add_to(at, weight_at[i]);
+      }
+    __syncthreads();
+    add_up(1, true, count, sum, list_of, list_to, list_sum);
+  };
+  auto open_list = [&](unsigned count, u64 sum) {
+    in_list = min((int)sh.listed, FS_LIST);
+    n_front = count;
+    front = sum;
+    unsigned low = 0xffffffffu, high = 0xffffffffu;                          // keys, the second from above
+#pragma unroll
+    for (int i = 0; i < FS_EACH; ++i) {
+      const int at = tid + i * FS_THREADS;
+      order_at[i] = weight_at[i] = 0;
+      if (at < in_list) {
+        order_at[i] = sh.list[at];
+        const unsigned key = (unsigned)(order_at[i] >> 32);
+        weight_at[i] = weight(fs_value(key));
+        low = min(low, key);
+        high = min(high, ~key);
+      }
+    }
+    if (in_list <= FS_FEW) {
+      if (tid < in_list) sh.list[FS_FEW + tid] = weight_at[0];
+      __syncthreads();
+      rank_few(in_list, n_front, front);
+    } else {
+      least = (u64)block.min(low) << 32;
+      most = (u64)~block.min(high) << 32 | 0xffffffffu;
+      cut_list(least, most, n_front, front);
+    }
+  };
+  auto find_in_list = [&](const Goal& goal) {
+    if (in_list <= FS_FEW) return first_ranked(in_list, goal);
+    if (cut_low != least || cut_high != most) cut_list(least, most, n_front, front);
+    while (true) {
+      const int at = min(FS_BINS - 1, first_of([&](int i) { return list_of[i] > 0 && goal.reached(list_to[i], list_sum[i]); }));
+      const int here = (int)at_place(list_of, at);
+      const unsigned count = (unsigned)at_place(list_to, at) - here;
+      const u64 sum = at > 0 ? at_place(list_sum, at - 1) : cut_sum;
+      const u64 high = cut_high - ((u64)at << cut_shift), span = (1ull << cut_shift) - 1;
+      const u64 low = high - cut_low > span ? high - span : cut_low;
+      if (here <= FS_FEW) {
+        if (tid == 0) sh.mine = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < FS_EACH; ++i)
+          if (tid + i * FS_THREADS < in_list && order_at[i] >= low && order_at[i] <= high) {
+            const unsigned to = atomicAdd(&sh.mine, 1u);
+            sh.list[to] = order_at[i];
+            sh.list[FS_FEW + to] = weight_at[i];
+          }
+        __syncthreads();
+        rank_few(here, count, sum);
+        return first_ranked(here, goal);
+      }
+      cut_list(low, high, count, sum);
+    }
+  };
+
+  // ---- 3 and 5. the first block decides what comes next, until the draw is found ----
+  const double u = u_asked >= 0.f ? fmin((double)u_asked, 1.0 - 1.0 / 16777216) : 0.0;
+  // An edge's weight from the single-precision exponential is off by less than 2^-16 of itself at the exponents that count, what
+  // a place is rounded by included.
+  const float step_log2 = bin_scale > 0.f ? (float)(1.0 / (double)bin_scale * rate) : 0.f;
+  enum : int { kTopK, kNucleus, kDraw };
+  int step = kTopK, end = 0, cut_by = 0;         // cut_by: what the threads' counts and sums are of (0: of nothing that serves)
+  bool listed = false, open = false, k_cuts = false;
+  unsigned count = 0;                            // in front of what was asked for, and their sum
+  u64 sum = 0, kept = 0;                         // the sum of what is kept so far
+  Goal k_goal{true, false, 0.0};
+  FsCommand c{};
+  c.what = count_only ? FS_COUNTS : FS_SUMS;
+  c.is_first = 1;
+  while (true) {
+    serve(c);
+    fs_sync();                                   // it has been carried out
+    if (rank != 0) {
+      if (c.is_last) return;
+      fs_sync();                                 // a command is there
+      c = sh.command;
+      continue;
+    }
+    if (c.what <= FS_RADIX) {
+      add_up(size, c.what != FS_COUNTS, count, sum, count_of, count_to, sum_to);
+      cut_by = c.what;
+      if (c.is_first) {
+        const unsigned candidates = (unsigned)at_place(count_to, FS_BINS - 1);
+        k_cuts = by_k && (unsigned)k_asked < candidates;
+        k_goal.goal = (double)(k_cuts ? (unsigned)k_asked : candidates);
+        if (!count_only) kept = at_place(sum_to, FS_BINS - 1);
+        // the last bin that can hold a kept candidate: top-k's, the nucleus' (where what it is a share of is known), min-p's (where
+        // nothing behind it is needed), the last one; and whether all up to it fit the list
+        const double p_goal = p_share * (double)kept;
+        end = first_of([&](int i) {
+          return k_goal.reached(count_to[i], 0) || (by_p && !by_k && (double)sum_to[i] >= p_goal) ||
+                 (by_m && !(by_k && by_p) && (double)exp2f(-(float)(tid * FS_EACH + i + 1) * step_log2) * (1 + 1.0 / 16384) < m_border);
+        });
+        listed = at_place(count_to, end) <= FS_LIST;
+      }
+    } else {
+      open_list(count, sum);
+      open = true;
+    }
+    while (true) {
+      if ((step == kTopK && !(listed ? by_k : k_cuts)) || (step == kNucleus && !by_p)) { ++step; continue; }
+      if (step == kDraw && by_m && (open || !listed)) {
+        u64 m_sum = 0;
+        if (listed) {
+#pragma unroll
+          for (int i = 0; i < FS_EACH; ++i)
+            if (tid + i * FS_THREADS < in_list && weight.plain(fs_value((unsigned)(order_at[i] >> 32))) >= m_border) m_sum += weight_at[i];
+          m_sum = block.sum(m_sum);
+        } else {
+          for (unsigned r = 0; r < size; ++r) m_sum += sh.sums[r].x;
+        }
+        kept = min(kept, m_sum);
+      }
+      const Goal goal = step == kTopK ? k_goal : Goal{false, step == kDraw, (step == kDraw ? u : p_share) * (double)kept};
+      if (open) {
+        const Found found = find_in_list(goal);
+        if (step == kDraw) {
+          if (tid == 0) out[row] = (int)~(unsigned)found.order;
+          return;
+        }
+        kept = step == kTopK ? found.sum : min(kept, found.sum);
+        ++step;
+        open = listed;
+        if (cut_by == FS_RADIX) cut_by = 0;
+        continue;
+      }
+      c.is_first = 0;
+      c.is_last = listed || step == kDraw;
+      if (listed) {
+        c.what = FS_FETCH;
+        c.first = 0;
+        c.last = end;
+        count = 0;
+        sum = 0;
+      } else if (cut_by != FS_SUMS && cut_by != FS_RADIX) {
+        c.what = FS_SUMS;
+        c.is_last = 0;
+        count = 0;
+        sum = 0;
+      } else {
+        const int at = min(FS_BINS - 1, first_of([&](int i) { return count_of[i] > 0 && goal.reached(count_to[i], sum_to[i]); }));
+        const unsigned here = (unsigned)at_place(count_of, at);
+        count = (unsigned)at_place(count_to, at) - here;
+        if (at > 0) sum = at_place(sum_to, at - 1);
+        else if (cut_by == FS_SUMS) sum = 0;
+        if (cut_by == FS_RADIX) {
+          const u64 span = (1ull << c.shift) - 1;
+          c.high -= (u64)at << c.shift;
+          c.low = c.high - c.low > span ? c.high - span : c.low;
+          c.what = here > FS_LIST ? FS_RADIX : FS_FETCH_ORDER;
+        } else if (here > FS_LIST) {             // from the whole order on
+          c.what = FS_RADIX;
+          c.low = (u64)fs_key(all.min) << 32;
+          c.high = (u64)fs_key(all.max) << 32 | 0xffffffffu;
+          count = 0;
+          sum = 0;
+        } else {
+          c.what = FS_FETCH;
+          c.first = c.last = at;
+        }
+        c.shift = fs_shift(c.high - c.low);
+        if (c.what == FS_RADIX) c.is_last = 0;
+      }
+      break;
+    }
     __syncthreads();
     if (warp == 0) {
       const uint4* words = reinterpret_cast<const uint4*>(&c);
@@ -496,244 +693,7 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
       if (lane == 0) sh.listed = 0;
     }
     fs_sync();
-    serve(c);
-    fs_sync();
-  };
-  auto total_of = [&](int which) {
-    u64 v = 0;
-    for (unsigned r = 0; r < size; ++r) v += which ? sh.sums[r].y : sh.sums[r].x;
-    return v;
-  };
-  // every bin's count over the cluster, and running counts; bounds on running sums, in units
-  unsigned count_of[FS_EACH], count_to[FS_EACH];
-  double least_to[FS_EACH], most_to[FS_EACH];
-  auto counts = [&]() {
-    uint4 v[FS_MAX_CLUSTER];
-#pragma unroll
-    for (int r = 0; r < FS_MAX_CLUSTER; ++r)
-      v[r] = r < (int)size ? fs_load128(&sh.count[tid * FS_EACH], r) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-    for (int i = 0; i < FS_EACH; ++i) count_of[i] = 0;
-#pragma unroll
-    for (int r = 0; r < FS_MAX_CLUSTER; ++r) { count_of[0] += v[r].x; count_of[1] += v[r].y; count_of[2] += v[r].z; count_of[3] += v[r].w; }
-  };
-  counts();
-  const u64 all_sum = by_k ? 0 : total_of(0), m_sum0 = by_k || !by_m ? 0 : total_of(1);
-  // An edge's weight in units from the single-precision exponential, widened by 2^-14 of itself (its own error, and what a place
-  // is rounded by, are below 2^-16 at the exponents that count); the last bin has no lower edge, nor has any where all
-  // candidates are equal or almost.
-  const float nats = bin_scale > 0.f ? 1.f / bin_scale : 0.f, step = (float)(nats * rate);
-  auto edge = [&](int b) { return b == 0 ? 1.f : exp2f(-(float)b * step); };
-  {
-    unsigned n_to = 0;
-    double least = 0, most = 0;
-    float high = edge(tid * FS_EACH);
-#pragma unroll
-    for (int i = 0; i < FS_EACH; ++i) {
-      const int b = tid * FS_EACH + i;
-      const float low = b == FS_BINS - 1 || !(step > 0.f) ? 0.f : edge(b + 1);
-      n_to += count_of[i];
-      most += count_of[i] * (fmin((double)high * (1 + 1.0 / 16384), 1.0) * weight.unit + 1);
-      least += count_of[i] * fmax((double)low * (1 - 1.0 / 16384) * weight.unit - 1, 0.0);
-      count_to[i] = n_to;
-      least_to[i] = least;
-      most_to[i] = most;
-      high = step > 0.f ? low : 1.f;
-    }
-    block.before(n_to, least, most);
-#pragma unroll
-    for (int i = 0; i < FS_EACH; ++i) { count_to[i] += n_to; least_to[i] += least; most_to[i] += most; }
   }
-  // the first of all places (a thread has four) whose test holds; FS_BINS if none does
-  auto first_of = [&](auto holds) {
-    unsigned at = FS_BINS;
-#pragma unroll
-    for (int i = FS_EACH - 1; i >= 0; --i)
-      if (holds(i)) at = tid * FS_EACH + i;
-    return (int)block.min(at);
-  };
-  // a number that the threads have four of, at a place
-  auto at_place = [&](const auto& v, int b) {
-    u64 mine = 0;
-#pragma unroll
-    for (int i = 0; i < FS_EACH; ++i)
-      if ((b & (FS_EACH - 1)) == i) mine = (u64)v[i];
-    return block.from(tid == b / FS_EACH, mine);
-  };
-  // The list, sorted, with its weights' running sums (from `front` on).
-  u64 sum_to[FS_EACH], order_at[FS_EACH];
-  int in_list = 0;
-  auto sorted = [&](u64 front) {
-    in_list = min((int)sh.listed, FS_LIST);
-    int padded = 128;
-    while (padded < in_list) padded <<= 1;
-#pragma unroll
-    for (int i = 0; i < FS_EACH; ++i) order_at[i] = tid * FS_EACH + i < in_list ? sh.list[tid * FS_EACH + i] : 0;
-    fs_sort(order_at, sh.list, padded);
-    u64 mine = 0;
-    if (warp * 32 * FS_EACH < in_list) {
-#pragma unroll
-      for (int i = 0; i < FS_EACH; ++i) {
-        if (tid * FS_EACH + i < in_list) mine += weight(fs_value((unsigned)(order_at[i] >> 32)));
-        sum_to[i] = mine;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < FS_EACH; ++i) sum_to[i] = 0;
-    }
-    unsigned none = 0, also_none = 0;
-    block.before(mine, none, also_none);
-#pragma unroll
-    for (int i = 0; i < FS_EACH; ++i) sum_to[i] += mine + front;
-  };
-  auto in_the_list = [&](int i) { return tid * FS_EACH + i < in_list; };
-  auto id_at = [&](int at) { return (int)~(unsigned)at_place(order_at, at); };
-
-  // The border of `goal`: makes the list hold the candidates around it, and returns the first place in the list that reaches
-  // it: the goal-th candidate (by_count), or the first whose running sum is > goal (strict) or >= goal.
-  auto border = [&](bool by_count, double goal, bool strict, bool want_m) {
-    auto reached = [&](double sum) { return strict ? sum > goal : sum >= goal; };
-    int first, last;
-    if (by_count) {
-      first = last = first_of([&](int i) { return (double)count_to[i] >= goal; });
-    } else {
-      first = first_of([&](int i) { return count_of[i] > 0 && most_to[i] * (1 + 1e-9) >= goal; });
-      last = min(FS_BINS - 1, first_of([&](int i) { return least_to[i] * (1 - 1e-9) > goal; }));
-      first = min(first, last);
-    }
-    unsigned passed = first > 0 ? (unsigned)at_place(count_to, first - 1) : 0;      // candidates in front of the list
-    const unsigned inside = (unsigned)at_place(count_to, last) - passed;
-    FsCommand c{};
-    c.what = FS_FETCH;
-    c.first = first;
-    c.last = last;
-    c.want_front = 1;
-    if (inside > FS_LIST) {
-      // cut finer: by the place below the largest, then by the order itself
-      unsigned kept_count[FS_EACH], kept_to[FS_EACH];
-#pragma unroll
-      for (int i = 0; i < FS_EACH; ++i) { kept_count[i] = count_of[i]; kept_to[i] = count_to[i]; }
-      c.what = FS_FINE;
-      c.fine_scale = 2047.96875f / (float)(last - first + 1);
-      u64 low = (u64)fs_key(all.min) << 32, high = (u64)fs_key(all.max) << 32 | 0xffffffffu;
-      while (true) {
-        if (c.what == FS_RADIX) {
-          c.low = low;
-          c.high = high;
-          c.shift = 0;
-          while ((high - low) >> c.shift >= FS_BINS) ++c.shift;
-        }
-        ask(c);
-        u64 before = total_of(0), sum = 0, to[FS_EACH];
-        counts();
-        for (unsigned r = 0; r < size; ++r) {
-          const uint4 a = fs_load128(reinterpret_cast<unsigned*>(sh.list) + tid * FS_EACH, r);
-          const uint4 b = fs_load128(reinterpret_cast<unsigned*>(sh.list) + FS_BINS + tid * FS_EACH, r);
-          const u64 w[FS_EACH] = {a.x + ((u64)b.x << 32), a.y + ((u64)b.y << 32), a.z + ((u64)b.z << 32), a.w + ((u64)b.w << 32)};
-#pragma unroll
-          for (int i = 0; i < FS_EACH; ++i) to[i] = (r ? to[i] : 0) + w[i];
-        }
-        unsigned n_to = 0, none = 0;
-#pragma unroll
-        for (int i = 0; i < FS_EACH; ++i) {
-          n_to += count_of[i];
-          count_to[i] = n_to;
-          sum += to[i];
-          to[i] = sum;
-        }
-        block.before(n_to, sum, none);
-#pragma unroll
-        for (int i = 0; i < FS_EACH; ++i) { count_to[i] += n_to; to[i] += sum + before; }
-        const unsigned in_front = passed;
-        const int at = min(FS_BINS - 1, first_of([&](int i) {
-          return count_of[i] > 0 && (by_count ? (double)(in_front + count_to[i]) >= goal : reached((double)to[i]));
-        }));
-        const unsigned here = (unsigned)at_place(count_of, at), in_bins = at > 0 ? (unsigned)at_place(count_to, at - 1) : 0;
-        if (c.what == FS_FINE) {
-          if (here <= FS_LIST) {
-            c.what = FS_FETCH_FINE;
-            c.fine = at;
-            passed += in_bins;
-            break;
-          }
-          c.what = FS_RADIX;                        // from the whole order on
-          passed = 0;
-        } else {
-          const u64 span = (1ull << c.shift) - 1;
-          high -= (u64)at << c.shift;
-          low = high - low > span ? high - span : low;
-          passed += in_bins;
-          if (here <= FS_LIST) {
-            c.what = FS_FETCH_ORDER;
-            c.low = low;
-            c.high = high;
-            break;
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < FS_EACH; ++i) { count_of[i] = kept_count[i]; count_to[i] = kept_to[i]; }
-    }
-    c.want_m = want_m;
-    c.is_last = strict;                             // the draw is the last border
-    ask(c);
-    sorted(total_of(0));
-    const unsigned in_front = passed;
-    const int at = first_of([&](int i) {
-      return in_the_list(i) && (by_count ? (double)(in_front + tid * FS_EACH + i + 1) >= goal : reached((double)sum_to[i]));
-    });
-    return max(0, min(at, in_list - 1));
-  };
-
-  const double u = u_asked >= 0.f ? fmin((double)u_asked, 1.0 - 1.0 / 16777216) : 0.0;
-  int chosen;
-  const unsigned candidates = (unsigned)at_place(count_to, FS_BINS - 1);
-  const bool k_cuts = by_k && (unsigned)k_asked < candidates;
-  // the last bin that can hold a kept candidate: top-k's, the nucleus' (where its sum is known), min-p's (where top-k and top-p do
-  // not need what lies behind it), the last one; and whether all up to it fit the list
-  const unsigned k_goal = k_cuts ? (unsigned)k_asked : candidates;
-  const double p_goal = p_share * (double)all_sum;
-  const int end = first_of([&](int i) {
-    return count_to[i] >= k_goal || (by_p && !by_k && least_to[i] >= p_goal) ||
-           (by_m && !(by_k && by_p) && (double)edge(tid * FS_EACH + i + 1) * (1 + 1.0 / 16384) < m_border);
-  });
-  if (at_place(count_to, end) <= FS_LIST) {
-    FsCommand c{};
-    c.what = FS_FETCH;
-    c.last = end;
-    c.is_last = 1;
-    ask(c);
-    sorted(0);
-    int kept = in_list;
-    if (k_cuts) kept = min(kept, k_asked);
-    if (by_p) {
-      const double goal = p_share * (double)(by_k ? at_place(sum_to, kept - 1) : all_sum);
-      kept = min(kept, first_of([&](int i) { return in_the_list(i) && (double)sum_to[i] >= goal; }) + 1);
-    }
-    if (by_m) {
-      const int below = first_of([&](int i) { return in_the_list(i) && weight.plain(fs_value((unsigned)(order_at[i] >> 32))) < m_border; });
-      kept = max(1, min(kept, below));
-    }
-    const double goal = u * (double)at_place(sum_to, kept - 1);
-    const int at = first_of([&](int i) { return in_the_list(i) && (double)sum_to[i] > goal; });
-    chosen = id_at(min(at, kept - 1));
-  } else {
-    u64 kept = all_sum, m_kept = m_sum0;
-    if (by_k) {
-      // the sum of the first k (of all where there are fewer)
-      const int at = border(true, (double)k_goal, false, by_m);
-      kept = at_place(sum_to, at);
-      if (by_m) m_kept = total_of(1);
-    }
-    if (by_p) {
-      const int at = border(false, p_share * (double)kept, false, false);
-      const u64 cut = at_place(sum_to, at);
-      kept = min(kept, cut);
-    }
-    if (by_m) kept = min(kept, m_kept);
-    chosen = id_at(border(false, u * (double)kept, true, false));
-  }
-  if (tid == 0) out[row] = chosen;
 }
 
 // Blocks a cluster: a row's slices stay in shared memory, two blocks a multiprocessor, up to 8 * 21,000 logits; few rows
