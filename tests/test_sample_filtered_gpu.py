@@ -100,6 +100,16 @@ def test_unusual_rows(what, vocab):
     compare(logits, temperature, top_k, top_p, min_p, u)
 
 
+@pytest.mark.parametrize("top_k", [0, 3000])
+@pytest.mark.parametrize("vocab", [2500, 9000, 40001])
+def test_a_nucleus_that_ends_behind_what_min_p_keeps(vocab, top_k):
+    """min-p keeps some hundred to two thousand candidates, the nucleus would keep more."""
+    rng = np.random.default_rng(vocab)
+    n = 24
+    logits = rng.normal(size=(n, vocab))
+    compare(logits, np.full(n, 1.3), np.full(n, top_k), rng.uniform(0.8, 0.9999, n), 10 ** rng.uniform(-2.0, -0.7, n), rng.random(n).astype(np.float32))
+
+
 def test_edges_of_the_settings():
     logits = np.tile(np.log(np.array([4.0, 2.0, 1.0, 1.0])), (12, 1))
     one, half = 1.0, 0.5

@@ -58,10 +58,13 @@ __device__ __forceinline__ unsigned fs_peer(const void* local, unsigned rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(theirs) : "r"((unsigned)__cvta_generic_to_shared(local)), "r"(rank));
   return theirs;
 }
-__device__ __forceinline__ uint2 fs_load64(const void* local, unsigned rank) {
-  uint2 v;
-  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(fs_peer(local, rank)));
+__device__ __forceinline__ unsigned fs_load32(const void* local, unsigned rank) {      // no memory clobber: several may be on their way
+  unsigned v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(fs_peer(local, rank)));
   return v;
+}
+__device__ __forceinline__ void fs_store32(const void* local, unsigned rank, unsigned v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(fs_peer(local, rank)), "r"(v) : "memory");
 }
 __device__ __forceinline__ void fs_store128(const void* local, unsigned rank, uint4 v) {
   asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};"
@@ -113,6 +116,8 @@ __device__ __forceinline__ int fs_shift(u64 range) { return max(0, 53 - __clzll(
 struct FsShared {
   u64 list[FS_LIST];                 // candidates; the sums of bins take the same place, low words and high words
   unsigned count[FS_BINS];
+  unsigned all_count[FS_BINS];       // the first block's: counts and sums of the whole row
+  u64 all_sum[FS_BINS];
   FsCommand command;
   FsStats stats[FS_MAX_CLUSTER];     // of the cluster's blocks, each written by its block
   uint4 ids[FS_MAX_CLUSTER];         // the first block's: the first id with the largest logit in each block's slice (x)
@@ -148,12 +153,12 @@ struct FsBlock {
     __syncthreads();
     return __reduce_min_sync(0xffffffffu, at[threadIdx.x & (FS_WARPS - 1)]);
   }
-  // the one thread's value whose test holds
-  __device__ __forceinline__ u64 from(bool mine, u64 v) {
+  // the one thread's values whose test holds
+  __device__ __forceinline__ ulonglong2 from(bool mine, u64 v, u64 w = 0) {
     u64* at = next();
-    if (mine) at[0] = v;
+    if (mine) { at[0] = v; at[1] = w; }
     __syncthreads();
-    return at[0];
+    return make_ulonglong2(at[0], at[1]);
   }
   // the count and the sum of the threads in front of this one, added to `count` and `sum`
   __device__ __forceinline__ void before(unsigned n, u64 v, unsigned& count, u64& sum) {
@@ -399,44 +404,42 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
       __syncthreads();
       const unsigned mine = min(sh.mine, (unsigned)FS_LIST);
       if (mine) {                                  // the same for the block
-        const u64 base = block.from(tid == 0, tid == 0 ? fs_add32(&sh.listed, 0, mine) : 0u);
+        const u64 base = block.from(tid == 0, tid == 0 ? fs_add32(&sh.listed, 0, mine) : 0u).x;
         for (unsigned i = tid; i < mine; i += FS_THREADS)
           if (base + i < FS_LIST) fs_store64(&sh.list[base + i], 0, sh.list[i]);
       }
     }
   };
-  // counts and sums of the thread's bins over `blocks` blocks, then running ones, from `front` on
+  // What has been cut, added up over the cluster into the first block's shared memory: a block has every size-th part of the
+  // bins, a thread two blocks' counts and sums of one (the first block alone, reading them all, was bound by what one
+  // multiprocessor takes in from others, 15 bytes a cycle: 5.9 us for counts and sums of 8 blocks, 2 with this).
+  auto gather = [&](bool sums) {
+    const int halves = size / 2, bin = rank * (FS_BINS / size) + tid / halves, r = tid % halves * 2;
+    unsigned n = fs_load32(&sh.count[bin], r) + fs_load32(&sh.count[bin], r + 1);
+    u64 v = 0;
+    if (sums) {
+      const unsigned low0 = fs_load32(low_word + bin, r), low1 = fs_load32(low_word + bin, r + 1);
+      const unsigned high0 = fs_load32(high_word + bin, r), high1 = fs_load32(high_word + bin, r + 1);
+      v = (u64)low0 + low1 + ((u64)(high0 + high1) << 32);
+    }
+    for (int o = 1; o < halves; o <<= 1) {
+      n += __shfl_xor_sync(0xffffffffu, n, o);
+      v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
+    if (r == 0) {
+      fs_store32(&sh.all_count[bin], 0, n);
+      if (sums) fs_store64(&sh.all_sum[bin], 0, v);
+    }
+  };
+  // the thread's bins of that (or of this block's own), and running ones behind `n_front` candidates of sum `front`
   unsigned count_of[FS_EACH] = {}, count_to[FS_EACH] = {};
   u64 sum_to[FS_EACH] = {};
-  auto add_up = [&](unsigned blocks, bool sums, unsigned n_front, u64 front, unsigned (&of)[FS_EACH], unsigned (&to)[FS_EACH], u64 (&sum)[FS_EACH]) {
+  auto add_up = [&](bool own, bool sums, unsigned n_front, u64 front, unsigned (&of)[FS_EACH], unsigned (&to)[FS_EACH], u64 (&sum)[FS_EACH]) {
 #pragma unroll
-    for (int i = 0; i < FS_EACH; ++i) { of[i] = 0; sum[i] = 0; }
-    // all loads of four blocks are asked for before the first is used (one behind the other they took 1.4 us each); a block that
-    // is not there: the first one's, which count for nothing
-#pragma unroll
-    for (unsigned r0 = 0; r0 < FS_MAX_CLUSTER; r0 += 4) {
-      if (r0 >= blocks) break;
-      uint2 n[4], a[4], b[4];
-#pragma unroll
-      for (unsigned e = 0; e < 4; ++e) n[e] = fs_load64(&sh.count[tid * FS_EACH], r0 + e < blocks ? r0 + e : 0);
-      if (sums) {
-#pragma unroll
-        for (unsigned e = 0; e < 4; ++e) {
-          a[e] = fs_load64(low_word + tid * FS_EACH, r0 + e < blocks ? r0 + e : 0);
-          b[e] = fs_load64(high_word + tid * FS_EACH, r0 + e < blocks ? r0 + e : 0);
-        }
-      }
-#pragma unroll
-      for (unsigned e = 0; e < 4; ++e) {
-        if (r0 + e < blocks) {
-          of[0] += n[e].x;
-          of[1] += n[e].y;
-          if (sums) {
-            sum[0] += a[e].x + ((u64)b[e].x << 32);
-            sum[1] += a[e].y + ((u64)b[e].y << 32);
-          }
-        }
-      }
+    for (int i = 0; i < FS_EACH; ++i) {
+      const int at = tid * FS_EACH + i;
+      of[i] = own ? sh.count[at] : sh.all_count[at];
+      sum[i] = !sums ? 0 : own ? low_word[at] + ((u64)high_word[at] << 32) : sh.all_sum[at];
     }
     to[0] = of[0];
 #pragma unroll
@@ -453,13 +456,26 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
       if (holds(i)) at = tid * FS_EACH + i;
     return (int)block.min(at);
   };
-  // a number that the threads have FS_EACH of, at a place
+  // of numbers that the threads have FS_EACH of, the one at a place
   auto at_place = [&](const auto& v, int b) {
     u64 mine = 0;
 #pragma unroll
     for (int i = 0; i < FS_EACH; ++i)
       if ((b & (FS_EACH - 1)) == i) mine = (u64)v[i];
-    return block.from(tid == b / FS_EACH, mine);
+    return block.from(tid == b / FS_EACH, mine).x;
+  };
+  // what bin b holds: its count, and count and sum of what lies in front of it
+  struct Bin { unsigned here, count; u64 sum; };
+  auto bin_at = [&](const unsigned (&of)[FS_EACH], const unsigned (&to)[FS_EACH], const u64 (&sum)[FS_EACH], int b, u64 none) {
+    const bool mine = tid == b / FS_EACH, before = tid == (b - 1) / FS_EACH && b > 0;
+    u64* at = block.next();
+#pragma unroll
+    for (int i = 0; i < FS_EACH; ++i) {
+      if (mine && (b & (FS_EACH - 1)) == i) at[0] = (u64)(to[i] - of[i]) << 32 | of[i];
+      if (before && ((b - 1) & (FS_EACH - 1)) == i) at[1] = sum[i];
+    }
+    __syncthreads();
+    return Bin{(unsigned)at[0], (unsigned)(at[0] >> 32), b > 0 ? at[1] : none};
   };
 
   // A goal: the goal-th candidate of the order (by_count), or the first whose running sum is > goal (strict) or >= goal.
@@ -490,13 +506,11 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
       }
     }
   };
-  // among n ranked ones
-  auto first_ranked = [&](int n, const Goal& goal) {
-    const unsigned at = block.min(tid < n && goal.reached(rank_at, ranked_sum) ? rank_at : 0xffffffffu);
-    const unsigned most = block.min(tid < n ? ~rank_at : 0xffffffffu);       // none reaches it: the last one
-    const bool mine = tid < n && rank_at == (at == 0xffffffffu ? ~most : at);
-    const u64 sum = block.from(mine, ranked_sum);
-    return Found{sum, block.from(mine, ranked)};
+  // among n ranked ones behind `count` others (where none reaches the goal: the last one)
+  auto first_ranked = [&](int n, unsigned count, const Goal& goal) {
+    const unsigned at = min(block.min(tid < n && goal.reached(rank_at, ranked_sum) ? rank_at : 0xffffffffu), count + n);
+    const ulonglong2 found = block.from(tid < n && rank_at == at, ranked_sum, ranked);
+    return Found{found.x, found.y};
   };
   // a longer one: cut into 2,048 parts of its order (or of low..high of it, behind `count` candidates of sum `sum`)
   unsigned list_of[FS_EACH], list_to[FS_EACH];
@@ -518,7 +532,7 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
         add_to(at, weight_at[i]);
       }
     __syncthreads();
-    add_up(1, true, count, sum, list_of, list_to, list_sum);
+    add_up(true, true, count, sum, list_of, list_to, list_sum);
   };
   auto open_list = [&](unsigned count, u64 sum) {
     in_list = min((int)sh.listed, FS_LIST);
@@ -548,16 +562,16 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
     }
   };
   auto find_in_list = [&](const Goal& goal) {
-    if (in_list <= FS_FEW) return first_ranked(in_list, goal);
+    if (in_list <= FS_FEW) return first_ranked(in_list, n_front, goal);
     if (cut_low != least || cut_high != most) cut_list(least, most, n_front, front);
     while (true) {
-      const int at = min(FS_BINS - 1, first_of([&](int i) { return list_of[i] > 0 && goal.reached(list_to[i], list_sum[i]); }));
-      const int here = (int)at_place(list_of, at);
-      const unsigned count = (unsigned)at_place(list_to, at) - here;
-      const u64 sum = at > 0 ? at_place(list_sum, at - 1) : cut_sum;
+      const int at = first_of([&](int i) { return list_of[i] > 0 && goal.reached(list_to[i], list_sum[i]); });
+      // a nucleus that ends behind what min-p keeps: all of the list
+      if (at >= FS_BINS) return Found{at_place(list_sum, FS_BINS - 1), 0};
+      const Bin bin = bin_at(list_of, list_to, list_sum, at, cut_sum);
       const u64 high = cut_high - ((u64)at << cut_shift), span = (1ull << cut_shift) - 1;
       const u64 low = high - cut_low > span ? high - span : cut_low;
-      if (here <= FS_FEW) {
+      if (bin.here <= FS_FEW) {
         if (tid == 0) sh.mine = 0;
         __syncthreads();
 #pragma unroll
@@ -568,10 +582,10 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
             sh.list[FS_FEW + to] = weight_at[i];
           }
         __syncthreads();
-        rank_few(here, count, sum);
-        return first_ranked(here, goal);
+        rank_few((int)bin.here, bin.count, bin.sum);
+        return first_ranked((int)bin.here, bin.count, goal);
       }
-      cut_list(low, high, count, sum);
+      cut_list(low, high, bin.count, bin.sum);
     }
   };
 
@@ -592,6 +606,10 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
   while (true) {
     serve(c);
     fs_sync();                                   // it has been carried out
+    if (c.what <= FS_RADIX && size > 1) {
+      gather(c.what != FS_COUNTS);
+      fs_sync();
+    }
     if (rank != 0) {
       if (c.is_last) return;
       fs_sync();                                 // a command is there
@@ -599,7 +617,7 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
       continue;
     }
     if (c.what <= FS_RADIX) {
-      add_up(size, c.what != FS_COUNTS, count, sum, count_of, count_to, sum_to);
+      add_up(size == 1, c.what != FS_COUNTS, count, sum, count_of, count_to, sum_to);
       cut_by = c.what;
       if (c.is_first) {
         const unsigned candidates = (unsigned)at_place(count_to, FS_BINS - 1);
@@ -661,16 +679,15 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
         sum = 0;
       } else {
         const int at = min(FS_BINS - 1, first_of([&](int i) { return count_of[i] > 0 && goal.reached(count_to[i], sum_to[i]); }));
-        const unsigned here = (unsigned)at_place(count_of, at);
-        count = (unsigned)at_place(count_to, at) - here;
-        if (at > 0) sum = at_place(sum_to, at - 1);
-        else if (cut_by == FS_SUMS) sum = 0;
+        const Bin bin = bin_at(count_of, count_to, sum_to, at, cut_by == FS_SUMS ? 0 : sum);
+        count = bin.count;
+        sum = bin.sum;
         if (cut_by == FS_RADIX) {
           const u64 span = (1ull << c.shift) - 1;
           c.high -= (u64)at << c.shift;
           c.low = c.high - c.low > span ? c.high - span : c.low;
-          c.what = here > FS_LIST ? FS_RADIX : FS_FETCH_ORDER;
-        } else if (here > FS_LIST) {             // from the whole order on
+          c.what = bin.here > FS_LIST ? FS_RADIX : FS_FETCH_ORDER;
+        } else if (bin.here > FS_LIST) {             // from the whole order on
           c.what = FS_RADIX;
           c.low = (u64)fs_key(all.min) << 32;
           c.high = (u64)fs_key(all.max) << 32 | 0xffffffffu;
@@ -696,9 +713,16 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
   }
 }
 
-// Blocks a cluster: a row's slices stay in shared memory, two blocks a multiprocessor, up to 8 * 21,000 logits; few rows
-// want many short slices, each a chain of passes.
-static int fs_cluster(int vocab) { return vocab > 24576 ? 8 : vocab > 8192 ? 4 : vocab > 3000 ? 2 : 1; }
+// Blocks a cluster.  A block has a multiprocessor to itself, and the device holds some 16 clusters of 8 or 34 of 4 at once: few
+// rows are cut into 8 slices, many into 2.  Slices below some 3,000 logits are not worth an exchange.  us for 8 / 4 / 2 / 1
+// blocks, rows with settings of their own: 152,064 logits, 8 rows 46 / 57 / 94 / 160, 24 58 / 57 / 88 / 141, 64 117 / 97 / 131 / 217; 49,999, 8
+// rows 36 / 37 / 46 / 71, 37 65 / 54 / 63 / 97, 64 88 / 58 / 62 / 98 (from a nucleus 108 / 64 / 43 / 63); 10,007, 37 rows 57 / 40 / 40 / 42; 2,000,
+// 8 rows 23 / 22 / 21 / 21.
+static int fs_cluster(int n_rows, int vocab) {
+  const int by_rows = n_rows <= 15 ? 8 : n_rows <= (vocab > 100000 ? 68 : 34) ? 4 : 2;
+  const int by_slice = vocab > 24576 ? 8 : vocab > 8192 ? 4 : vocab > 3000 ? 2 : 1;
+  return by_rows < by_slice ? by_rows : by_slice;
+}
 
 // Draws one id a row of `logits` [n_rows][vocab].  `top_k` (0 or less: off), `top_p` (1 or more: off) and `min_p` (0: off) may be
 // null; `uniform` holds numbers from [0, 1).
@@ -707,9 +731,9 @@ TOKB200_API int tokb200_sample_filtered(const float* logits, int n_rows, int voc
                                         cudaStream_t stream) {
   if (n_rows <= 0) return TOKB200_OK;
   if (vocab <= 0 || n_rows > (1 << 27)) return TOKB200_BAD_SIZE;
-  const int cluster = fs_cluster(vocab);
+  const int cluster = fs_cluster(n_rows, vocab);
   const int slice = (vocab + cluster - 1) / cluster;
-  constexpr size_t kMost = 200 * 1024;               // of a block's shared memory
+  constexpr size_t kMost = 224 * 1024;               // of a block's shared memory
   const size_t held = ((size_t)slice + 8) * 4;       // in groups of four, of which the first and the last may be cut
   const bool resident = sizeof(FsShared) + held <= kMost;
   const size_t smem = sizeof(FsShared) + (resident ? held : 0);
