@@ -9,9 +9,12 @@
 //    the rows of q are gathered by threads, and what a block leaves is a part: weighted values, maximum and sum in 32 bits.
 //    The keys are cut into as many pieces as fill the device once.
 // 2. The own keys on mma.sync, and the join.  A cluster of blocks a (row, key/value head): each block walks a piece of the row's
-//    own keys, the group's heads as one product (a warp takes 32 keys a turn, the next tile's keys and values on their way
-//    meanwhile); the pieces meet in distributed shared memory, and each block joins every size-th head with the parts of
-//    the first kernel.
+//    own keys, the group's heads as one product (a warp takes 32 keys a turn; the next keys are asked for when the scores are
+//    computed, the next values when the weighted sum is); the pieces meet in distributed shared memory, and each block joins
+//    every size-th head with the parts of the first kernel.
+// The first kernel lets the second start at once: what it reads but the parts (rows, tables, q, keys and values) was complete
+// before the first kernel began, which starts strictly behind its predecessor.  Its blocks take the multiprocessors that the
+// first kernel leaves and those that it has done with, and wait for it only in front of the join.
 #define FA_WAIT_LIMIT (1u << 17)      // polls of up to 20 us each: seconds in all
 #ifndef HEAD_DIM
 #define HEAD_DIM 64
@@ -35,9 +38,11 @@ constexpr int kPFirst = kPOnScores ? 0 : 256 + HEAD_DIM;
 constexpr int kHalfKeys = SP_KEYS / 2;            // of a block, that a softmax thread owns
 constexpr int kTileBytes = kDBlocks * kSubTile;
 constexpr int kStatBytes = 2 * 2 * SP_ROWS * 4;
-constexpr int kBarBytes = (2 * SP_BUFFERS + 6) * 8 + 8;     // the barriers, where tensor memory lies, whether a wait ran out
+constexpr int kBarBytes = (2 * SP_BUFFERS + 7) * 8 + 8;     // the barriers, where tensor memory lies, whether a wait ran out
 constexpr int kFaSmem = 2 * kTileBytes + SP_BUFFERS * kTileBytes + kStatBytes + kBarBytes;
 static_assert(kFaSmem > 116 * 1024 && kFaSmem <= 227 * 1024, "one block an SM: it takes all of tensor memory");
+constexpr int kOutStride = HEAD_DIM * 4 + 16;     // bytes between the rows of a part on their way out through the ring's memory
+static_assert(2 * SP_ROWS * kOutStride <= SP_BUFFERS * kTileBytes, "the rows of two lanes fit the ring");
 
 #include "fa_tcgen05.cuh"
 
@@ -67,7 +72,8 @@ shared_prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __
   unsigned long long* s_full = empty + SP_BUFFERS;               // [2], commit of Q K^T
   unsigned long long* p_ready = s_full + 2;                      // [2], an arrival per softmax warp of the lane
   unsigned long long* pv_done = p_ready + 2;                     // [2], commit of P V
-  unsigned* tmem_slot = reinterpret_cast<unsigned*>(pv_done + 2);
+  unsigned long long* q_full = pv_done + 2;                      // an arrival a softmax warp
+  unsigned* tmem_slot = reinterpret_cast<unsigned*>(q_full + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int piece = blockIdx.x, kvh = blockIdx.y, group = nh / nkv;
@@ -84,6 +90,7 @@ shared_prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __
       fa_mbar_init(&p_ready[i], SP_SOFTMAX_WARPS / 2);
       fa_mbar_init(&pv_done[i], 1);
     }
+    fa_mbar_init(q_full, SP_SOFTMAX_WARPS);
     tmem_slot[1] = 0;                            // no wait has run out
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -93,6 +100,7 @@ shared_prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait();
+  pdl_launch();
   const int4 tile = tiles[blockIdx.z];
   const int lead = tile.y > 0 ? members[tile.x] : -1;
   const int req = lead < 0 ? -1 : row_req[lead];
@@ -120,17 +128,6 @@ shared_prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __
   auto block_at = [&](int n) { return !split ? n / 2 : n < 2 ? n : n % 2 == 0 ? n / 2 - 1 : (n + 1) / 2; };
   const int* table = block_table + (size_t)(live ? req : 0) * table_stride;
 
-  if (live) {
-    // the rows of q, 16 bytes a thread; rows behind the members: zeros
-    for (int i = threadIdx.x; i < (split ? 1 : 2) * SP_ROWS * (HEAD_DIM / 8); i += SP_THREADS) {
-      const int c = i % (HEAD_DIM / 8), r = i / (HEAD_DIM / 8) % SP_ROWS, l = i / (HEAD_DIM / 8) / SP_ROWS;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      const int row = r < rows_of(l) ? member_of(l, r) : -1;
-      if (row >= 0) v = *reinterpret_cast<const uint4*>(q + ((size_t)row * nh + kvh * group + r % group) * HEAD_DIM + c * 8);
-      *reinterpret_cast<uint4*>(q_s + l * kTileBytes + (c / 8) * kSubTile + swz(r, c % 8)) = v;
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -228,7 +225,7 @@ shared_prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __
       }
       __syncwarp();
     };
-    bool ok = true;
+    bool ok = wait(q_full, 0);
     for (int l = 0; ok && l < 2; ++l)
       if (steps_of(l) > 0 && (ok = wait_place(k_place(block_of(l, 0))))) scores(l, 0);
     const int most = steps_of(0);
@@ -266,6 +263,27 @@ shared_prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __
     float* my_stat = stat_s + (l * 2 + half) * SP_ROWS + r;
     const float* other_stat = stat_s + (l * 2 + 1 - half) * SP_ROWS + r;
     auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + l * 4 + (warp & 3)) : "memory"); };
+    const int row = r < rows_of(l) ? member_of(l, r) : -1;
+    if (!split || l == 0) {
+      // the rows of q that the warp's lanes own, half of a row's lanes a warp, 16 bytes a load; behind the members: zeros
+      constexpr int kPieces = HEAD_DIM / 16, kRowsAtOnce = 32 / kPieces;
+      uint4 v[32 / kRowsAtOnce];
+#pragma unroll
+      for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
+        const int in_warp = i * kRowsAtOnce + lane / kPieces, from = __shfl_sync(0xffffffffu, row, in_warp);
+        const int head = kvh * group + ((warp & 3) * 32 + in_warp) % group;
+        v[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (from >= 0) v[i] = *reinterpret_cast<const uint4*>(q + ((size_t)from * nh + head) * HEAD_DIM + (half * kPieces + lane % kPieces) * 8);
+      }
+#pragma unroll
+      for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
+        const int at = (warp & 3) * 32 + i * kRowsAtOnce + lane / kPieces, c = half * kPieces + lane % kPieces;
+        *reinterpret_cast<uint4*>(q_s + l * kTileBytes + (c / 8) * kSubTile + swz(at, c % 8)) = v[i];
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncwarp();
+    if (lane == 0) fa_mbar_arrive(q_full);
     const int steps = steps_of(l);
     float m_ref = -INFINITY, l_run = 0.f;     // reference maximum (raw score units, the row's) and running sum (this half's)
     bool ok = true;
@@ -360,13 +378,15 @@ shared_prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __
       weight_other = m_other == -INFINITY ? 0.f : fa_exp2((m_other - m_all) * scale_log2);
       den = (steps > 0 ? weight * l_all : 0.f) + (other_steps > 0 ? weight_other * l_other : 0.f);
     }
-    const int row = r < rows_of(l) ? member_of(l, r) : -1;
+    // The part leaves through the ring's memory (both lanes' products have read all of it), a thread's run of a row in one bulk
+    // copy: stored from registers, 16 bytes a row and instruction, 256 rows took 4 us.
+    if (!split) asm volatile("bar.sync 9, %0;" ::"n"(SP_SOFTMAX_WARPS * 32) : "memory");
     if (__all_sync(0xffffffffu, ok)) {
       // a thread writes its half of the head; split, its quarter, from both accumulators (one without a step was never written)
       const int width = split ? HEAD_DIM / 4 : HEAD_DIM / 2, from = (split ? l * 2 + half : half) * width;
       const size_t at = ((size_t)max(row, 0) * nh + kvh * group + r % group) * pieces + piece;
       if (row >= 0 && half == 0 && (!split || l == 0)) stat_parts[at] = make_float2(m_all * scale_log2, den);
-      float* dst = acc_parts + at * HEAD_DIM;
+      unsigned char* out_row = ring + (split ? r : l * SP_ROWS + r) * kOutStride;
 #pragma unroll 1
       for (int c0 = from; c0 < from + width; c0 += 16) {
         float acc[16];
@@ -384,18 +404,20 @@ shared_prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __
 #pragma unroll
           for (int i = 0; i < 16; ++i) acc[i] = fmaf(weight_other, part[i], acc[i]);
         }
-        if (row >= 0) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            reinterpret_cast<float4*>(dst + c0)[c] = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
-        }
+        for (int c = 0; c < 4; ++c)
+          *reinterpret_cast<float4*>(out_row + (c0 + 4 * c) * 4) = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (row >= 0)
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
+                     ::"l"(acc_parts + at * HEAD_DIM + from), "r"(fa_smem(out_row + from * 4)), "r"(width * 4) : "memory");
+      asm volatile("cp.async.bulk.commit_group;\ncp.async.bulk.wait_group 0;" ::: "memory");
     }
   }
   // ---------------- common exit ----------------
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  pdl_launch();
   if (threadIdx.x == 0 && tmem_slot[1] != 0) {
     atomicExch(&sp_error_flag, 1);
     tokb200_report_error(TOKB200_LIB_SHARED_PREFIX_TCGEN05, 1);
@@ -413,8 +435,8 @@ shared_prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __
 #define OWN_MAX_GROUP 16              // heads of a group: the rows of one mma
 #define OWN_MAX_CLUSTER 8
 constexpr int kSteps = HEAD_DIM / 32;                // steps of 32 lanes of the head: one 16-byte load, two mma
-constexpr int kVStride = HEAD_DIM + 8;               // elements between staged value rows
-constexpr int kRow = HEAD_DIM + 2;                   // a part in shared memory: weighted values, maximum (log2 units), sum
+constexpr int kOwnStride = HEAD_DIM + 8;             // elements between staged rows of keys and of values
+constexpr int kRow = HEAD_DIM + 4;                   // a part in shared memory: weighted values, maximum (log2 units), sum
 
 __device__ __forceinline__ void own_mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
   asm volatile(
@@ -433,75 +455,69 @@ __device__ __forceinline__ unsigned own_pack(float lo, float hi) {
 __device__ __forceinline__ void own_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
-// a float of block `rank` of this cluster, at the place `local` has in this block's shared memory
-__device__ __forceinline__ float own_peer(const float* local, unsigned rank) {
+// four floats of block `rank` of this cluster, at the place `local` has in this block's shared memory (no memory clobber: several
+// may be on their way)
+__device__ __forceinline__ float4 own_peer(const float* local, unsigned rank) {
   unsigned theirs;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(theirs) : "r"(fa_smem(local)), "r"(rank));
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(theirs) : "memory");
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(theirs));
   return v;
 }
 // lanes of the head that thread t of a quad reads in step st: a permutation that q and keys share, which a dot product does
 // not see; a quad's two pieces of 16 bytes lie side by side
 __device__ __forceinline__ int own_lane(int st, int t) { return (st >> 1) * 64 + 16 * t + 8 * (st & 1); }
 
-__global__ void __launch_bounds__(OWN_THREADS, HEAD_DIM == 64 ? 4 : 2)
+// `alone`: no first kernel runs in front of this one
+__global__ void __launch_bounds__(OWN_THREADS, 3)
 shared_prefix_own_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ k_pool,
                          const __nv_bfloat16* __restrict__ v_pool, __nv_bfloat16* __restrict__ out,
                          const int* __restrict__ block_table, int table_stride, const int* __restrict__ row_req,
                          const int* __restrict__ pos, const int* __restrict__ shared, int nh, int nkv, int page, int tile_pieces,
-                         float scale, const float* __restrict__ sink, float softcap, const float* __restrict__ acc_parts,
+                         float scale, const float* __restrict__ sink, float softcap, int alone, const float* __restrict__ acc_parts,
                          const float2* __restrict__ stat_parts) {
   const int rank = blockIdx.x, size = gridDim.x, kvh = blockIdx.y, row = blockIdx.z;
   const int group = nh / nkv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  pdl_wait();
-  pdl_launch();
+  if (alone) pdl_wait();
   const int req = row_req[row];
-  if (req < 0) return;                               // the same for the whole cluster
+  if (req < 0) {                                     // the same for the whole cluster
+    if (!alone) pdl_wait();
+    pdl_launch();
+    return;
+  }
   const int reach = table_stride * page, common = min(max(shared[row], 0), reach);
   const int n_own = max(min(pos[row] + 1, reach) - common, 0);
   const int len = ((n_own + size - 1) / size + OWN_TILE - 1) / OWN_TILE * OWN_TILE;
   const int first = common + rank * len, last = common + min(n_own, (rank + 1) * len) - 1;     // none: last < first
   const int n_tile = common > 0 ? (common + sp_piece(common, tile_pieces) - 1) / sp_piece(common, tile_pieces) : 0;
   const int* table = block_table + (size_t)req * table_stride;
-  __nv_bfloat16* v_buf = reinterpret_cast<__nv_bfloat16*>(fa_raw) + (size_t)warp * 2 * OWN_TILE * kVStride;
+  __nv_bfloat16* k_s = reinterpret_cast<__nv_bfloat16*>(fa_raw) + (size_t)warp * 2 * OWN_TILE * kOwnStride;
+  __nv_bfloat16* v_s = k_s + OWN_TILE * kOwnStride;
 
   const int page_shift = (page & (page - 1)) == 0 ? __ffs(page) - 1 : -1;
-  auto tile_slots = [&](int k0) {
+  auto tile_slots = [&](int k0) {                    // a key a lane
     const int key = k0 + lane;
     if (key > last) return -1;
     const int pg = page_shift >= 0 ? key >> page_shift : key / page;
     return max(table[pg], 0) * page + (key - pg * page);
   };
-  auto stage_values = [&](int my_slot, __nv_bfloat16* dst_rows) {
-    constexpr int kPieces = HEAD_DIM / 8;   // 16-byte pieces a row
+  // a tile's rows, 16 bytes a copy, a row's pieces side by side; rows behind the last key: zeros
+  auto stage = [&](int my_slot, const __nv_bfloat16* pool, __nv_bfloat16* dst_rows) {
+    constexpr int kPieces = HEAD_DIM / 8;
 #pragma unroll
     for (int c = 0; c < kPieces; ++c) {
       const int i = c * 32 + lane, at = i / kPieces, piece = i % kPieces;
       const int slot = __shfl_sync(0xffffffffu, my_slot, at);
-      fa_copy16(dst_rows + at * kVStride + piece * 8, v_pool + ((size_t)max(slot, 0) * nkv + kvh) * HEAD_DIM + piece * 8, slot >= 0);
+      fa_copy16(dst_rows + at * kOwnStride + piece * 8, pool + ((size_t)max(slot, 0) * nkv + kvh) * HEAD_DIM + piece * 8, slot >= 0);
     }
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
-  uint4 kf[OWN_TILE / 8][kSteps];
-  auto load_keys = [&](int my_slot) {
-#pragma unroll
-    for (int nt = 0; nt < OWN_TILE / 8; ++nt) {
-      const int slot = __shfl_sync(0xffffffffu, my_slot, nt * 8 + g);
-      const __nv_bfloat16* k_row = k_pool + ((size_t)max(slot, 0) * nkv + kvh) * HEAD_DIM;
-#pragma unroll
-      for (int st = 0; st < kSteps; ++st)
-        kf[nt][st] = slot >= 0 ? *reinterpret_cast<const uint4*>(k_row + own_lane(st, t)) : make_uint4(0u, 0u, 0u, 0u);
-    }
-  };
-  int turn = 0;
   const int k_mine = first + warp * OWN_TILE;
-  int slots_now = -1;
   if (k_mine <= last) {
-    slots_now = tile_slots(k_mine);
-    stage_values(slots_now, v_buf);
-    load_keys(slots_now);
+    const int slots = tile_slots(k_mine);
+    stage(slots, k_pool, k_s);
+    stage(slots, v_pool, v_s);
   }
   unsigned qa[kSteps][2][4];
   {
@@ -523,22 +539,27 @@ shared_prefix_own_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat1
   const float scale_log2 = scale * 1.4426950408889634f;
   const bool capped = softcap > 0.f;
   const float cap_in = capped ? scale / softcap : 0.f, cap_out = softcap * 1.4426950408889634f;
-  for (int k0 = k_mine; k0 <= last; k0 += OWN_WARPS * OWN_TILE, turn ^= 1) {
-    __nv_bfloat16* v_s = v_buf + (size_t)turn * OWN_TILE * kVStride;
-    const bool more = k0 + OWN_WARPS * OWN_TILE <= last;
-    const int slots_next = more ? tile_slots(k0 + OWN_WARPS * OWN_TILE) : -1;
-    if (more) stage_values(slots_next, v_buf + (size_t)(turn ^ 1) * OWN_TILE * kVStride);
+#pragma unroll 1
+  for (int k0 = k_mine; k0 <= last; k0 += OWN_WARPS * OWN_TILE) {
+    const int k_next = k0 + OWN_WARPS * OWN_TILE;
+    const bool more = k_next <= last;
+    const int slots_next = more ? tile_slots(k_next) : -1;
+    asm volatile("cp.async.wait_group 1;\n" ::: "memory");     // this tile's keys have landed (its values may not)
+    __syncwarp();
     float s[OWN_TILE / 8][4];
 #pragma unroll
     for (int nt = 0; nt < OWN_TILE / 8; ++nt) {
       s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      const __nv_bfloat16* k_row = k_s + (nt * 8 + g) * kOwnStride;
 #pragma unroll
       for (int st = 0; st < kSteps; ++st) {
-        own_mma(s[nt], qa[st][0], kf[nt][st].x, kf[nt][st].y);
-        own_mma(s[nt], qa[st][1], kf[nt][st].z, kf[nt][st].w);
+        const uint4 kf = *reinterpret_cast<const uint4*>(k_row + own_lane(st, t));
+        own_mma(s[nt], qa[st][0], kf.x, kf.y);
+        own_mma(s[nt], qa[st][1], kf.z, kf.w);
       }
     }
-    if (more) load_keys(slots_next);
+    __syncwarp();
+    if (more) stage(slots_next, k_pool, k_s);
     float m_new[2] = {m_run[0], m_run[1]};
 #pragma unroll
     for (int nt = 0; nt < OWN_TILE / 8; ++nt)
@@ -576,7 +597,7 @@ shared_prefix_own_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat1
       o[i][0] *= corr[0]; o[i][1] *= corr[0];
       o[i][2] *= corr[1]; o[i][3] *= corr[1];
     }
-    if (more) asm volatile("cp.async.wait_group 1;\n" ::: "memory");   // this tile's values have landed (the next tile's may not)
+    if (more) asm volatile("cp.async.wait_group 1;\n" ::: "memory");   // this tile's values have landed (the next keys may not)
     else asm volatile("cp.async.wait_group 0;\n" ::: "memory");
     __syncwarp();
 #pragma unroll
@@ -589,12 +610,13 @@ shared_prefix_own_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat1
 #pragma unroll
       for (int dp = 0; dp < HEAD_DIM / 16; ++dp) {
         unsigned vf[4];
-        own_ldmatrix_x4_trans(vf, v_s + (ks * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * kVStride + dp * 16 + (lane >> 4) * 8);
+        own_ldmatrix_x4_trans(vf, v_s + (ks * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * kOwnStride + dp * 16 + (lane >> 4) * 8);
         own_mma(o[2 * dp], pf, vf[0], vf[1]);
         own_mma(o[2 * dp + 1], pf, vf[2], vf[3]);
       }
     }
-    __syncwarp();   // the staged values are overwritten by the next tile
+    __syncwarp();
+    if (more) stage(slots_next, v_pool, v_s);
   }
 
   // ---- the block's part: its warps' joined (the buffer takes the place of the staged values) ----
@@ -630,52 +652,86 @@ shared_prefix_own_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat1
     if (c == 0) { piece_s[(size_t)head * kRow + HEAD_DIM] = m; piece_s[(size_t)head * kRow + HEAD_DIM + 1] = den; }
   }
   if (size > 1) own_cluster_sync(); else __syncthreads();
-  // ---- every size-th head of the group: the pieces of the cluster's blocks and the parts of the common keys, a lane each ----
-  for (int head = rank + size * warp; head < group; head += size * OWN_WARPS) {
-    const float* piece = piece_s + (size_t)head * kRow;
-    const size_t at = ((size_t)row * nh + kvh * group + head) * tile_pieces;
-    float m = -INFINITY, l = 0.f;
-    if (lane < size) {
-      m = own_peer(piece + HEAD_DIM, (unsigned)lane);
-      l = own_peer(piece + HEAD_DIM + 1, (unsigned)lane);
-    } else if (lane - size < n_tile) {
-      const float2 v = __ldcg(&stat_parts[at + lane - size]);
-      m = v.x;
-      l = v.y;
-    }
-    const float m_all = warp_max(m), f = exp2f(m - m_all);
-    float den = warp_sum(f * l);
-    if (sink) den += exp2f(sink[kvh * group + head] * 1.4426950408889634f - m_all);
-    constexpr int kEach = HEAD_DIM / 32;                         // lanes of the head a thread
-    float num[kEach] = {};
-    for (int i = 0; i < size; ++i) {
-      const float w = __shfl_sync(0xffffffffu, f, i);
+  if (!alone) pdl_wait();                            // the parts of the common keys are there
+  pdl_launch();
+  // ---- every size-th head of the group, half a warp each: the pieces of the cluster's blocks and the parts of the common keys ----
+  const int n_parts = size + n_tile, hl = lane & 15;
+  for (int i0 = 2 * warp; rank + size * i0 < group; i0 += 2 * OWN_WARPS) {
+    const int head = rank + size * (i0 + (lane >> 4));
+    const bool on = head < group;
+    const float* piece = piece_s + (size_t)(on ? head : 0) * kRow;
+    const size_t at = ((size_t)row * nh + kvh * group + (on ? head : 0)) * tile_pieces;
+    // two parts a lane: their maxima, sums and weights
+    float m[2], l[2], f[2];
 #pragma unroll
-      for (int c = 0; c < kEach; ++c) num[c] = fmaf(w, own_peer(piece + lane * kEach + c, (unsigned)i), num[c]);
+    for (int e = 0; e < 2; ++e) {
+      const int i = hl + 16 * e;
+      m[e] = -INFINITY;
+      l[e] = 0.f;
+      if (i < size) {
+        const float4 v = size > 1 ? own_peer(piece + HEAD_DIM, (unsigned)i) : *reinterpret_cast<const float4*>(piece + HEAD_DIM);
+        m[e] = v.x;
+        l[e] = v.y;
+      } else if (i < n_parts) {
+        const float2 v = __ldcg(&stat_parts[at + i - size]);
+        m[e] = v.x;
+        l[e] = v.y;
+      }
+    }
+    float m_all = fmaxf(m[0], m[1]), den = 0.f;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, o));
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      f[e] = exp2f(m[e] - m_all);
+      den += hl + 16 * e < n_parts ? f[e] * l[e] : 0.f;
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+    if (sink && on) den += exp2f(sink[kvh * group + head] * 1.4426950408889634f - m_all);
+    constexpr int kQuads = HEAD_DIM / 64;                        // four lanes of the head at a time: hl and, of 128, hl + 16
+    float num[kQuads][4] = {};
+    auto weight_of = [&](int i) { return __shfl_sync(0xffffffffu, i < 16 ? f[0] : f[1], (lane & 16) | (i & 15)); };
+    auto add = [&](int k, float w, const float4& v) {
+      num[k][0] = fmaf(w, v.x, num[k][0]);
+      num[k][1] = fmaf(w, v.y, num[k][1]);
+      num[k][2] = fmaf(w, v.z, num[k][2]);
+      num[k][3] = fmaf(w, v.w, num[k][3]);
+    };
+    if (size == 1) {
+      const float w = weight_of(0);
+#pragma unroll
+      for (int k = 0; k < kQuads; ++k) add(k, w, *reinterpret_cast<const float4*>(piece + (hl + 16 * k) * 4));
+    } else {
+      for (int i = 0; i < size; i += 2) {                        // a power of two
+        float4 v[2][kQuads];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int k = 0; k < kQuads; ++k) v[e][k] = own_peer(piece + (hl + 16 * k) * 4, (unsigned)(i + e));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float w = weight_of(i + e);
+#pragma unroll
+          for (int k = 0; k < kQuads; ++k) add(k, w, v[e][k]);
+        }
+      }
     }
 #pragma unroll 4
     for (int i = 0; i < n_tile; ++i) {
-      const float w = __shfl_sync(0xffffffffu, f, size + i);
-      const float* src = acc_parts + (at + i) * HEAD_DIM + lane * kEach;
-      if (kEach == 4) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-        num[0] = fmaf(w, v.x, num[0]);
-        num[1] = fmaf(w, v.y, num[1]);
-        num[kEach - 2] = fmaf(w, v.z, num[kEach - 2]);
-        num[kEach - 1] = fmaf(w, v.w, num[kEach - 1]);
-      } else {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-        num[0] = fmaf(w, v.x, num[0]);
-        num[1] = fmaf(w, v.y, num[1]);
-      }
-    }
-    const float inv = n_tile + n_own > 0 ? 1.0f / den : 0.f;     // a row without a key: zeros
-    __nv_bfloat16* dst = out + ((size_t)row * nh + kvh * group + head) * HEAD_DIM + lane * kEach;
+      const float w = weight_of(size + i);
+      const float4* src = reinterpret_cast<const float4*>(acc_parts + (at + i) * HEAD_DIM);
 #pragma unroll
-    for (int c = 0; c < kEach; c += 2) {
-      const float a = n_tile + n_own > 0 ? num[c] * inv : 0.f, b = n_tile + n_own > 0 ? num[c + 1] * inv : 0.f;
-      *reinterpret_cast<unsigned*>(dst + c) = own_pack(a, b);
+      for (int k = 0; k < kQuads; ++k) add(k, w, __ldcg(src + hl + 16 * k));
     }
+    const bool any = n_tile + n_own > 0;                         // a row without a key: zeros
+    const float inv = any ? 1.0f / den : 0.f;
+    __nv_bfloat16* dst = out + ((size_t)row * nh + kvh * group + head) * HEAD_DIM;
+#pragma unroll
+    for (int k = 0; k < kQuads; ++k)
+      if (on)
+        *reinterpret_cast<uint2*>(dst + (hl + 16 * k) * 4) =
+            any ? make_uint2(own_pack(num[k][0] * inv, num[k][1] * inv), own_pack(num[k][2] * inv, num[k][3] * inv)) : make_uint2(0u, 0u);
   }
   if (size > 1) own_cluster_sync();                  // nobody leaves while its piece may still be read
 }
@@ -695,26 +751,28 @@ TOKB200_API int tokb200_shared_prefix_tcgen05_pieces(int n_rows, int n_tiles, in
   if (pieces > most) pieces = most;
   *tile_pieces = pieces < 1 ? 1 : pieces > SP_MAX_PIECES ? SP_MAX_PIECES : pieces;
   int own = 1;
-  while (own < OWN_MAX_CLUSTER && n_rows * nkv * own * 2 <= 4 * sms) own *= 2;
+  while (own < OWN_MAX_CLUSTER && n_rows * nkv * own * 2 <= 8 * sms) own *= 2;
   *own_pieces = own;
   return TOKB200_OK;
 }
 
-// As tokb200_shared_prefix_attention; acc_parts and stat_parts hold n_rows * nh * tile_pieces parts.
+// As tokb200_shared_prefix_attention; `parts` holds n_rows * nh * tile_pieces * (HEAD_DIM + 2) floats where there are tiles.
 TOKB200_API int tokb200_shared_prefix_tcgen05(
     const void* q, const void* k_pool, const void* v_pool, void* out, const int* block_table, int table_stride, const int* row_req,
     const int* pos, const int* shared, const int* members, const int* tiles, int n_tiles, int n_rows, int pool_rows, int nh, int nkv,
-    int d, int page, float scale, const float* sink, float softcap, int tile_pieces, int own_pieces, float* acc_parts,
-    float* stat_parts, cudaStream_t stream) {
+    int d, int page, float scale, const float* sink, float softcap, int tile_pieces, int own_pieces, float* parts,
+    cudaStream_t stream) {
   if (n_rows <= 0) return TOKB200_OK;
   if (d != HEAD_DIM || nh <= 0 || nkv <= 0 || nh % nkv || nh / nkv > OWN_MAX_GROUP || page <= 0 || page % 8 || pool_rows <= 0 || n_tiles < 0 ||
       n_tiles > 65535 || n_rows > 65535 || nkv > 65535 || table_stride <= 0 || (long long)table_stride * page > 0x7fffffffLL ||
-      tile_pieces < 1 || tile_pieces > SP_MAX_PIECES || own_pieces < 1 || own_pieces > OWN_MAX_CLUSTER)
+      tile_pieces < 1 || tile_pieces > SP_MAX_PIECES || own_pieces < 1 || own_pieces > OWN_MAX_CLUSTER || (own_pieces & (own_pieces - 1)))
     return TOKB200_BAD_SIZE;
-  if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out | (uintptr_t)tiles | (uintptr_t)acc_parts | (uintptr_t)stat_parts) & 15)
+  if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out | (uintptr_t)tiles | (uintptr_t)parts) & 15)
     return TOKB200_BAD_ALIGNMENT;
+  float* acc_parts = parts;                            // behind them the maxima and sums
+  float2* stat_parts = (float2*)(parts + (size_t)n_rows * nh * tile_pieces * HEAD_DIM);
   const int group = nh / nkv;
-  const size_t stage = (size_t)2 * OWN_WARPS * OWN_TILE * kVStride * sizeof(__nv_bfloat16);
+  const size_t stage = (size_t)2 * OWN_WARPS * OWN_TILE * kOwnStride * sizeof(__nv_bfloat16);
   const size_t merge = (size_t)(OWN_WARPS + 1) * group * kRow * sizeof(float);
   const size_t own_smem = stage > merge ? stage : merge;
   static bool configured[64] = {};
@@ -741,7 +799,7 @@ TOKB200_API int tokb200_shared_prefix_tcgen05(
                             dim3(tile_pieces, nkv, n_tiles), dim3(SP_THREADS), (size_t)kFaSmem, stream, map_k, map_v, (const __nv_bfloat16*)q,
                             (const __nv_bfloat16*)v_pool, block_table, table_stride, row_req, members, (const int4*)tiles, nh, nkv, page,
                             run, pool_rows, tile_pieces, scale * 1.4426950408889634f, softcap > 0.f ? scale / softcap : 0.f,
-                            softcap > 0.f ? softcap / scale : 0.f, acc_parts, (float2*)stat_parts);
+                            softcap > 0.f ? softcap / scale : 0.f, acc_parts, stat_parts);
     if (status != TOKB200_OK) return status;
   }
   cudaLaunchConfig_t config = {};
@@ -763,7 +821,7 @@ TOKB200_API int tokb200_shared_prefix_tcgen05(
   config.numAttrs = 2;
   const cudaError_t err = cudaLaunchKernelEx(&config, shared_prefix_own_kernel, (const __nv_bfloat16*)q, (const __nv_bfloat16*)k_pool,
                                              (const __nv_bfloat16*)v_pool, (__nv_bfloat16*)out, block_table, table_stride, row_req, pos, shared,
-                                             nh, nkv, page, tile_pieces, scale, sink, softcap, (const float*)acc_parts,
+                                             nh, nkv, page, tile_pieces, scale, sink, softcap, n_tiles > 0 ? 0 : 1, (const float*)acc_parts,
                                              (const float2*)stat_parts);
   return err == cudaSuccess ? TOKB200_OK : (int)err;
 }
