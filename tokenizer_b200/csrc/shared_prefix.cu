@@ -18,7 +18,8 @@
 #define SP_PAIRS_WARP 4
 #define SP_PAIRS (SP_WARPS * SP_PAIRS_WARP)       // (row, head) pairs of a block
 #define SP_KEYS 32
-#define SP_MIN_PIECE 64
+#define SP_MIN_PIECE 32
+#define SP_JOIN_THREADS 64
 #define SP_LOG2E 1.4426950408889634f
 
 // keys of a piece when n keys are cut into at most `pieces`
@@ -29,12 +30,12 @@ __host__ __device__ __forceinline__ int sp_piece(int n, int pieces) {
 
 // parts: [row][head][tile_pieces + own_pieces][d + 2]
 template <typename T, int DI>
-__global__ void __launch_bounds__(SP_THREADS)
+__global__ void __launch_bounds__(SP_THREADS, DI <= 4 ? 2 : 1)
 shared_prefix_parts_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, const T* __restrict__ v_pool,
                            const int* __restrict__ block_table, int table_stride, const int* __restrict__ row_req,
                            const int* __restrict__ pos, const int* __restrict__ shared, const int* __restrict__ members,
                            const int4* __restrict__ tiles, int n_tiles, int nh, int nkv, int d, int page, float scale_log2,
-                           float cap_in, float cap_out, int tile_pieces, int own_pieces, float* __restrict__ parts) {
+                           float cap_in, float cap_out, int tile_chunks, int row_chunks, int tile_pieces, int own_pieces, float* __restrict__ parts) {
   constexpr int kD = DI * 32, kStride = kD + 4;
   extern __shared__ __align__(16) float sp_smem[];
   float* q_s = sp_smem;                              // [pair][kD]
@@ -42,15 +43,18 @@ shared_prefix_parts_kernel(const T* __restrict__ q, const T* __restrict__ k_pool
   float* v_s = k_s + SP_KEYS * kStride;              // [key][kD]
   float4* p_s = reinterpret_cast<float4*>(v_s + SP_KEYS * kD);      // [warp][key]: the probabilities of a warp's pairs
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = nh / nkv, kvh = blockIdx.y % nkv, chunk = blockIdx.y / nkv, piece = blockIdx.x;
-  const bool common = (int)blockIdx.z < n_tiles;
+  // z: the tiles, each in chunks of SP_PAIRS pairs, then the rows
+  const int group = nh / nkv, kvh = blockIdx.y, piece = blockIdx.x;
+  const bool common = (int)blockIdx.z < n_tiles * tile_chunks;
+  const int unit = common ? blockIdx.z / tile_chunks : (blockIdx.z - n_tiles * tile_chunks) / row_chunks;
+  const int chunk = common ? blockIdx.z % tile_chunks : (blockIdx.z - n_tiles * tile_chunks) % row_chunks;
   pdl_wait();
   pdl_launch();
   // the block's pairs: (member, head) of a tile, or the heads of a row; its keys first..end of table `req`
   int first_member = 0, n_pairs, req, first, end, slot;
-  const int row_alone = common ? -1 : (int)blockIdx.z - n_tiles;
+  const int row_alone = common ? -1 : unit;
   if (common) {
-    const int4 tile = tiles[blockIdx.z];
+    const int4 tile = tiles[unit];
     const int lead = tile.y > 0 ? members[tile.x] : -1;
     first_member = tile.x;
     n_pairs = tile.y * group;
@@ -72,12 +76,21 @@ shared_prefix_parts_kernel(const T* __restrict__ q, const T* __restrict__ k_pool
   int row[SP_PAIRS_WARP], head[SP_PAIRS_WARP];
 #pragma unroll
   for (int i = 0; i < SP_PAIRS_WARP; ++i) {
-    const int in_block = warp * SP_PAIRS_WARP + i, pair = chunk * SP_PAIRS + in_block;
+    const int pair = chunk * SP_PAIRS + warp * SP_PAIRS_WARP + i;
     row[i] = pair < n_pairs ? row_of(pair) : -1;
     head[i] = kvh * group + pair % group;
-    const T* from = q + ((size_t)max(row[i], 0) * nh + head[i]) * d;
+  }
+  {
+    float v[SP_PAIRS_WARP][DI];
 #pragma unroll
-    for (int c = lane; c < kD; c += 32) q_s[in_block * kD + c] = row[i] >= 0 && c < d ? to_float(from[c]) : 0.f;
+    for (int i = 0; i < SP_PAIRS_WARP; ++i)
+#pragma unroll
+      for (int c = 0; c < DI; ++c)
+        v[i][c] = row[i] >= 0 && lane + 32 * c < d ? to_float(q[((size_t)row[i] * nh + head[i]) * d + lane + 32 * c]) : 0.f;
+#pragma unroll
+    for (int i = 0; i < SP_PAIRS_WARP; ++i)
+#pragma unroll
+      for (int c = 0; c < DI; ++c) q_s[(warp * SP_PAIRS_WARP + i) * kD + lane + 32 * c] = v[i][c];
   }
   float m_run[SP_PAIRS_WARP], l_run[SP_PAIRS_WARP], acc[SP_PAIRS_WARP][DI];
 #pragma unroll
@@ -88,20 +101,39 @@ shared_prefix_parts_kernel(const T* __restrict__ q, const T* __restrict__ k_pool
     for (int c = 0; c < DI; ++c) acc[i][c] = 0.f;
   }
   const int* table = block_table + (size_t)req * table_stride;
+  // a warp brings every eighth key of a tile; the next tile's rows are asked for while this one is computed
+  constexpr int kEach = SP_KEYS / SP_WARPS;
+  T k_next[kEach][DI], v_next[kEach][DI];
+  auto fetch = [&](int k0) {
+    int slot[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int key = k0 + e * SP_WARPS + warp;
+      slot[e] = key < end ? max(table[key / page], 0) * page + key % page : -1;
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const size_t at = ((size_t)max(slot[e], 0) * nkv + kvh) * d;
+#pragma unroll
+      for (int c = 0; c < DI; ++c) {                 // keys that are not seen, and lanes behind the head: zeros
+        const bool on = slot[e] >= 0 && lane + 32 * c < d;
+        k_next[e][c] = on ? k_pool[at + lane + 32 * c] : from_float<T>(0.f);
+        v_next[e][c] = on ? v_pool[at + lane + 32 * c] : from_float<T>(0.f);
+      }
+    }
+  };
+  fetch(first);
   for (int k0 = first; k0 < end; k0 += SP_KEYS) {
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < SP_KEYS / SP_WARPS; ++e) {
-      const int in_tile = e * SP_WARPS + warp, key = k0 + in_tile;
-      const bool on = key < end;
-      const size_t at = on ? ((size_t)max(table[key / page], 0) * page + key % page) * nkv + kvh : 0;
+    for (int e = 0; e < kEach; ++e)
 #pragma unroll
-      for (int c = lane; c < kD; c += 32) {          // keys that are not seen, and lanes behind the head: zeros
-        k_s[in_tile * kStride + c] = on && c < d ? to_float(k_pool[at * d + c]) : 0.f;
-        v_s[in_tile * kD + c] = on && c < d ? to_float(v_pool[at * d + c]) : 0.f;
+      for (int c = 0; c < DI; ++c) {
+        k_s[(e * SP_WARPS + warp) * kStride + lane + 32 * c] = to_float(k_next[e][c]);
+        v_s[(e * SP_WARPS + warp) * kD + lane + 32 * c] = to_float(v_next[e][c]);
       }
-    }
     __syncthreads();
+    if (k0 + SP_KEYS < end) fetch(k0 + SP_KEYS);
     float s[SP_PAIRS_WARP] = {};
     const float4* k_row = reinterpret_cast<const float4*>(k_s + lane * kStride);
 #pragma unroll 8
@@ -154,40 +186,45 @@ shared_prefix_parts_kernel(const T* __restrict__ q, const T* __restrict__ k_pool
   }
 }
 
-// a warp a (row, head)
-template <typename T>
-__global__ void __launch_bounds__(SP_THREADS)
+// a warp a (row, head), a part a lane for the weights
+template <typename T, int DI>
+__global__ void __launch_bounds__(SP_JOIN_THREADS)
 shared_prefix_join_kernel(const float* __restrict__ parts, const int* __restrict__ row_req, const int* __restrict__ pos,
                           const int* __restrict__ shared, int n_rows, int nh, int d, int reach, int tile_pieces, int own_pieces,
                           const float* __restrict__ sink, T* __restrict__ out) {
   pdl_wait();
   pdl_launch();
-  const int pair = blockIdx.x * SP_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int pair = blockIdx.x * (SP_JOIN_THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (pair >= n_rows * nh) return;
   const int row = pair / nh, head = pair % nh;
   if (row_req[row] < 0) return;
-  const int keys = min(max(shared[row], 0), reach), n = max(min(pos[row] + 1, reach) - max(shared[row], 0), 0);
-  const int n_tile = keys > 0 ? (keys + sp_piece(keys, tile_pieces) - 1) / sp_piece(keys, tile_pieces) : 0;
-  const int n_own = n > 0 ? (n + sp_piece(n, own_pieces) - 1) / sp_piece(n, own_pieces) : 0;
+  const int from = max(shared[row], 0), keys = min(from, reach), n = max(min(pos[row] + 1, reach) - from, 0);
+  const int tile_len = sp_piece(keys, tile_pieces), own_len = sp_piece(n, own_pieces);
+  const int n_tile = (keys + tile_len - 1) / tile_len, n_parts = n_tile + (n + own_len - 1) / own_len;      // at most a lane each
   const float* base = parts + (size_t)pair * (tile_pieces + own_pieces) * (d + 2);
   auto part_of = [&](int i) { return base + (size_t)(i < n_tile ? i : tile_pieces + i - n_tile) * (d + 2); };
-  float m = -INFINITY;
-  for (int i = lane; i < n_tile + n_own; i += 32) m = fmaxf(m, part_of(i)[d]);
-  m = warp_max(m);
-  float den = 0.f;
-  for (int i = lane; i < n_tile + n_own; i += 32) den += exp2f(part_of(i)[d] - m) * part_of(i)[d + 1];
-  den = warp_sum(den);
+  const bool on = lane < n_parts;
+  const float m_part = on ? part_of(lane)[d] : -INFINITY, l_part = on ? part_of(lane)[d + 1] : 0.f;
+  const float m = warp_max(m_part), f = exp2f(m_part - m);
+  float den = warp_sum(on ? f * l_part : 0.f);
   if (sink) den += exp2f(sink[head] * SP_LOG2E - m);
-  for (int c = lane; c < d; c += 32) {
-    float num = 0.f;
-    for (int i = 0; i < n_tile + n_own; ++i) num += exp2f(part_of(i)[d] - m) * part_of(i)[c];
-    out[(size_t)pair * d + c] = from_float<T>(n_tile + n_own ? num / den : 0.f);      // a row without a key: zeros
+  float num[DI] = {};
+#pragma unroll 8
+  for (int i = 0; i < n_parts; ++i) {
+    const float w = __shfl_sync(0xffffffffu, f, i);
+    const float* part = part_of(i);
+#pragma unroll
+    for (int c = 0; c < DI; ++c)
+      if (lane + 32 * c < d) num[c] = fmaf(w, part[lane + 32 * c], num[c]);
   }
+#pragma unroll
+  for (int c = 0; c < DI; ++c)
+    if (lane + 32 * c < d) out[(size_t)pair * d + lane + 32 * c] = from_float<T>(n_parts ? num[c] / den : 0.f);      // a row without a key: zeros
 }
 
 // (pieces of a tile's keys, pieces of a row's own keys) for a launch of these sizes: enough blocks for the device, at most 16
 TOKB200_API int tokb200_shared_prefix_pieces(int n_rows, int n_tiles, int nkv, int reach, int* tile_pieces, int* own_pieces) {
-  const int most = (reach + SP_MIN_PIECE - 1) / SP_MIN_PIECE, blocks = 148 * 4;
+  const int most = (reach + SP_MIN_PIECE - 1) / SP_MIN_PIECE, blocks = 148 * 4;      // together at most 32: a lane each in the join
   auto cut = [&](int units) {
     int n = units > 0 ? (blocks + units - 1) / units : 1;
     n = n > 16 ? 16 : n;
@@ -204,9 +241,10 @@ static int sp_launch(const void* q, const void* k_pool, const void* v_pool, void
                      int tile_members, int n_rows, int nh, int nkv, int d, int page, float scale, const float* sink, float softcap,
                      int tile_pieces, int own_pieces, float* parts, cudaStream_t stream) {
   const int group = nh / nkv;
-  const int most_pairs = (n_tiles > 0 && tile_members > 1 ? tile_members : 1) * group;
-  const int chunks = (most_pairs + SP_PAIRS - 1) / SP_PAIRS;
-  if ((long long)nkv * chunks > 65535 || n_tiles + n_rows > 65535) return TOKB200_BAD_SIZE;
+  const int members_most = tile_members < n_rows ? tile_members : n_rows;
+  const int tile_chunks = (members_most * group + SP_PAIRS - 1) / SP_PAIRS, row_chunks = (group + SP_PAIRS - 1) / SP_PAIRS;
+  const long long units = (long long)n_tiles * tile_chunks + (long long)n_rows * row_chunks;
+  if (nkv > 65535 || units > 65535) return TOKB200_BAD_SIZE;
   const size_t smem = (size_t)(SP_PAIRS * DI * 32 + SP_KEYS * (DI * 32 + 4) + SP_KEYS * DI * 32 + SP_WARPS * SP_KEYS * 4) * 4;
   static bool configured[64] = {};
   int device = 0;
@@ -216,14 +254,15 @@ static int sp_launch(const void* q, const void* k_pool, const void* v_pool, void
     if (err != cudaSuccess) return (int)err;
     configured[device] = true;
   }
-  const dim3 grid(tile_pieces > own_pieces ? tile_pieces : own_pieces, nkv * chunks, n_tiles + n_rows);
+  const dim3 grid(tile_pieces > own_pieces ? tile_pieces : own_pieces, nkv, (unsigned)units);
   int status = launch_dependent(shared_prefix_parts_kernel<T, DI>, grid, dim3(SP_THREADS), smem, stream, (const T*)q, (const T*)k_pool,
                                 (const T*)v_pool, block_table, table_stride, row_req, pos, shared, members, (const int4*)tiles, n_tiles, nh,
                                 nkv, d, page, scale * SP_LOG2E, softcap > 0.f ? scale / softcap : 0.f,
-                                softcap > 0.f ? softcap * SP_LOG2E : 0.f, tile_pieces, own_pieces, parts);
+                                softcap > 0.f ? softcap * SP_LOG2E : 0.f, tile_chunks, row_chunks, tile_pieces, own_pieces, parts);
   if (status != TOKB200_OK) return status;
-  return launch_dependent(shared_prefix_join_kernel<T>, dim3((unsigned)((n_rows * nh + SP_WARPS - 1) / SP_WARPS)), dim3(SP_THREADS), 0, stream,
-                          parts, row_req, pos, shared, n_rows, nh, d, table_stride * page, tile_pieces, own_pieces, sink, (T*)out);
+  constexpr int kPairs = SP_JOIN_THREADS / 32;
+  return launch_dependent(shared_prefix_join_kernel<T, DI>, dim3((unsigned)((n_rows * nh + kPairs - 1) / kPairs)), dim3(SP_JOIN_THREADS), 0,
+                          stream, parts, row_req, pos, shared, n_rows, nh, d, table_stride * page, tile_pieces, own_pieces, sink, (T*)out);
 }
 
 // tiles: [n_tiles][4] = (first place in `members`, members, keys, 0); at most `tile_members` members each.
@@ -233,7 +272,7 @@ TOKB200_API int tokb200_shared_prefix_attention(
     int n_rows, int nh, int nkv, int d, int page, float scale, const float* sink, float softcap, int tile_pieces, int own_pieces,
     float* parts, cudaStream_t stream) {
   if (n_rows <= 0) return TOKB200_OK;
-  if (nh <= 0 || nkv <= 0 || nh % nkv || d <= 0 || d > 256 || page <= 0 || n_tiles < 0 || tile_members < 0 || tile_pieces < 1 || own_pieces < 1 ||
+  if (nh <= 0 || nkv <= 0 || nh % nkv || d <= 0 || d > 256 || page <= 0 || n_tiles < 0 || tile_members < 1 || tile_pieces < 1 || own_pieces < 1 ||
       tile_pieces > 65535 || table_stride <= 0 || (long long)table_stride * page > 0x7fffffffLL || (long long)n_rows * nh > 0x7fffffffLL)
     return TOKB200_BAD_SIZE;
   if ((uintptr_t)tiles & 15) return TOKB200_BAD_ALIGNMENT;

@@ -486,7 +486,7 @@ shared_prefix_own_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat1
     pdl_launch();
     return;
   }
-  const int reach = table_stride * page, common = min(max(shared[row], 0), reach);
+  const int reach = table_stride * page, common = shared ? min(max(shared[row], 0), reach) : 0;
   const int n_own = max(min(pos[row] + 1, reach) - common, 0);
   const int len = ((n_own + size - 1) / size + OWN_TILE - 1) / OWN_TILE * OWN_TILE;
   const int first = common + rank * len, last = common + min(n_own, (rank + 1) * len) - 1;     // none: last < first
@@ -717,7 +717,7 @@ shared_prefix_own_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat1
         }
       }
     }
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < n_tile; ++i) {
       const float w = weight_of(size + i);
       const float4* src = reinterpret_cast<const float4*>(acc_parts + (at + i) * HEAD_DIM);
@@ -743,16 +743,19 @@ TOKB200_API int tokb200_shared_prefix_tcgen05_error(void) {
   return flag;
 }
 
-// (pieces of a tile's keys, blocks of a row's own keys) for a launch of these sizes
+// (pieces of a tile's keys, blocks of a row's own keys) for a launch of these sizes; no tiles: the rows' whole keys are their own.
 TOKB200_API int tokb200_shared_prefix_tcgen05_pieces(int n_rows, int n_tiles, int nkv, int reach, int* tile_pieces, int* own_pieces) {
-  const int sms = 148;
-  int pieces = n_tiles > 0 ? sms / (n_tiles * nkv) : 1;
-  const int most = (reach + SP_KEYS - 1) / SP_KEYS;
+  const int sms = 148, own_an_sm = 3;
+  const int units = n_rows * nkv;
+  int own = 1;
+  while (own < OWN_MAX_CLUSTER && (n_tiles > 0 ? units * own * 2 <= sms / 2 && own * 1024 <= reach : units * own * 2 <= own_an_sm * sms && own * 128 < reach))
+    own *= 2;
+  *own_pieces = own;
+  // the first kernel's blocks, one a multiprocessor, beside as many as the second one's take
+  const int tiles = n_tiles > 0 ? n_tiles * nkv : 1, left = sms - (units * own + own_an_sm - 1) / own_an_sm, most = (reach + SP_KEYS - 1) / SP_KEYS;
+  int pieces = (left > sms / 3 ? left : sms / 3) / tiles;
   if (pieces > most) pieces = most;
   *tile_pieces = pieces < 1 ? 1 : pieces > SP_MAX_PIECES ? SP_MAX_PIECES : pieces;
-  int own = 1;
-  while (own < OWN_MAX_CLUSTER && n_rows * nkv * own * 2 <= 8 * sms) own *= 2;
-  *own_pieces = own;
   return TOKB200_OK;
 }
 

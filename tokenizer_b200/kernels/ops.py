@@ -633,6 +633,12 @@ def shared_prefix_attention(q, k_pool, v_pool, out, block_table, row_req, pos, s
     # the parts are of this launch alone: captured graphs and streams share nothing
     if q.dtype == torch.bfloat16 and shared_prefix_tcgen05_supported(nh, nkv, d, page) and \
             (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr() | out.data_ptr()) % 16 == 0:
+        # Rows that have little to read altogether read all of it themselves, in one kernel (us, that / common keys apart, behind
+        # 14 heads over 2 of 64: 4 rows of 576 keys 5.0 / 10.1, 16 of 1,152 7.5 / 10.3, 64 of 640 (21 MB) 9.4 / 11.9, of 1,152 (38 MB)
+        # 12.0 / 11.2; 28 over 4 of 128: 8 of 640 9.4 / 11.4, 32 of 384 (25 MB) 12.0 / 12.7, 16 of 1,152 15.3 / 11.2; few rows of long
+        # reach have too few blocks: 2 of 2,176 11.6 / 11.6, of 4,224 16.0 / 13.0).
+        if rows * reach * nkv * d * 4 <= 24e6 and reach * d <= 300000:
+            n_tiles, shared = 0, None
         lib, tile_pieces, own_pieces = _shared_prefix_plan(d, rows, n_tiles, nkv, reach)
         parts = rows * nh * tile_pieces if n_tiles else 0
         scratch = torch.empty(parts * (d + 2), dtype=torch.float32, device=q.device)
