@@ -28,6 +28,12 @@ __host__ __device__ __forceinline__ int sp_piece(int n, int pieces) {
   return len < SP_MIN_PIECE ? SP_MIN_PIECE : len;
 }
 
+__device__ __forceinline__ float sp_warp_max(float v) {      // one instruction; NaN only if all are
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+
 // parts: [row][head][tile_pieces + own_pieces][d + 2]
 template <typename T, int DI>
 __global__ void __launch_bounds__(SP_THREADS, DI <= 4 ? 2 : 1)
@@ -134,7 +140,7 @@ shared_prefix_parts_kernel(const T* __restrict__ q, const T* __restrict__ k_pool
       }
     __syncthreads();
     if (k0 + SP_KEYS < end) fetch(k0 + SP_KEYS);
-    float s[SP_PAIRS_WARP] = {};
+    float part[2][SP_PAIRS_WARP] = {};               // two sums a score: half the chain of dependent additions
     const float4* k_row = reinterpret_cast<const float4*>(k_s + lane * kStride);
 #pragma unroll 8
     for (int c = 0; c < kD / 4; ++c) {
@@ -142,19 +148,21 @@ shared_prefix_parts_kernel(const T* __restrict__ q, const T* __restrict__ k_pool
 #pragma unroll
       for (int i = 0; i < SP_PAIRS_WARP; ++i) {
         const float4 qv = reinterpret_cast<const float4*>(q_s + (warp * SP_PAIRS_WARP + i) * kD)[c];
-        s[i] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s[i]))));
+        part[0][i] = fmaf(qv.x, kv.x, fmaf(qv.z, kv.z, part[0][i]));
+        part[1][i] = fmaf(qv.y, kv.y, fmaf(qv.w, kv.w, part[1][i]));
       }
     }
     float p[SP_PAIRS_WARP];
 #pragma unroll
     for (int i = 0; i < SP_PAIRS_WARP; ++i) {
-      float x = cap_out > 0.f ? cap_out * tanhf(s[i] * cap_in) : s[i] * scale_log2;
+      const float s = part[0][i] + part[1][i];
+      float x = cap_out > 0.f ? cap_out * tanhf(s * cap_in) : s * scale_log2;
       if (k0 + lane >= end) x = -INFINITY;
-      const float m_new = fmaxf(m_run[i], warp_max(x));
+      const float m_new = fmaxf(m_run[i], sp_warp_max(x));
       // a part whose scores are all -inf so far has no weight yet (a NaN among them goes through)
       const float corr = m_new == -INFINITY ? 1.f : exp2f(m_run[i] - m_new);
       p[i] = x == -INFINITY ? 0.f : exp2f(x - m_new);
-      l_run[i] = l_run[i] * corr + warp_sum(p[i]);
+      l_run[i] = l_run[i] * corr + p[i];             // of this lane's keys
       m_run[i] = m_new;
 #pragma unroll
       for (int c = 0; c < DI; ++c) acc[i][c] *= corr;
@@ -177,12 +185,13 @@ shared_prefix_parts_kernel(const T* __restrict__ q, const T* __restrict__ k_pool
   }
 #pragma unroll
   for (int i = 0; i < SP_PAIRS_WARP; ++i) {
+    const float l_all = warp_sum(l_run[i]);
     if (row[i] < 0) continue;
     float* part = parts + (((size_t)row[i] * nh + head[i]) * (tile_pieces + own_pieces) + slot) * (d + 2);
 #pragma unroll
     for (int c = 0; c < DI; ++c)
       if (lane + 32 * c < d) part[lane + 32 * c] = acc[i][c];
-    if (lane == 0) { part[d] = m_run[i]; part[d + 1] = l_run[i]; }
+    if (lane == 0) { part[d] = m_run[i]; part[d + 1] = l_all; }
   }
 }
 
