@@ -6,6 +6,7 @@ from typing import List
 
 import torch
 
+from ..kernels import ops
 from ..parts.base import CacheBinding, Runtime
 from .manager import CachePlan, RequestCache
 
@@ -50,6 +51,14 @@ class DeviceCache(CachePlan):
         if cache.length:            # a request that is recomputed from its first token starts from zero
             for arena in self._arenas():
                 arena[cache.state_slot].zero_()
+
+    def on_fork(self, parent: RequestCache, children: List[RequestCache], copies) -> None:
+        with torch.cuda.device(self.runtime.device):
+            for pool, pairs in zip(self.pools, copies):
+                ops.copy_pages(pool, self.page_size, pairs)
+            slots = [(parent.state_slot, child.state_slot, 1) for child in children]
+            for arena in self._arenas():               # a row of state a slot
+                ops.copy_pages(arena.view(1, arena.shape[0], 1, -1), 1, slots)
 
     def bindings(self, order) -> List[CacheBinding]:
         """One binding per call of the order."""

@@ -201,6 +201,45 @@ class CachePlan:
         cache.length = len(shared) * self.page_size
         return cache.length
 
+    # ---- forks ----------------------------------------------------------------------
+    def can_fork(self, parent: RequestCache) -> int:
+        """How many forks of `parent` the request slots and the pages allow now."""
+        most = len(self._free_slots)
+        if parent.length % self.page_size:
+            most = min([most] + [a.available for a in self.allocators])
+        return most
+
+    def fork(self, parent: RequestCache, request_ids: Sequence[object]) -> List[RequestCache]:
+        """Open requests that hold what `parent` holds: its full pages, shared (a page that a window gave back stays a
+        hole), a copy of the page that it has begun, and its state.  All or nothing: OutOfPages leaves everything as it
+        was."""
+        ids = list(request_ids)
+        if parent.closed:
+            raise ValueError("the request is closed")
+        if len(set(ids)) < len(ids) or any(i in self.requests for i in ids):
+            raise ValueError("a fork has a request id of its own")
+        if len(ids) > self.can_fork(parent):
+            raise OutOfPages(f"{len(ids)} forks of request {parent.request_id!r}: slots and pages are left for {self.can_fork(parent)}")
+        full, begun = divmod(parent.length, self.page_size)
+        children = [self.open(i) for i in ids]
+        copies: List[List[tuple]] = [[] for _ in self.groups]       # per group (page, its copy, rows)
+        for child in children:
+            child.length, child.published = parent.length, parent.published
+            for g, allocator in enumerate(self.allocators):
+                child.tables[g] = list(parent.tables[g][:full])
+                for page in child.pages_held(g):
+                    allocator.hold(page)
+        for child in children:
+            for g, allocator in enumerate(self.allocators):
+                if begun:
+                    child.tables[g].append(allocator.take())
+                    copies[g].append((parent.tables[g][full], child.tables[g][full], begun))
+        self.on_fork(parent, children, copies)
+        return children
+
+    def on_fork(self, parent: RequestCache, children: List[RequestCache], copies: List[List[tuple]]) -> None:
+        """Hook for the device side (copying the begun pages and the state)."""
+
     def publish_prompt(self, cache: RequestCache, tokens: Sequence[int]) -> None:
         """Offer the full pages that hold `tokens` (the beginning of the request's prompt, as far
         as it is computed) to later requests.  Called again with more of the same prompt, only

@@ -33,13 +33,15 @@ class GenerateParams:
     seed: int = 0
     eos: Sequence[int] = ()
     stop: Sequence[str] = ()
+    top_k: int = 0             # the first k candidates (0: all); top_p is then a share of what they weigh
+    min_p: float = 0.0         # candidates that weigh at least this share of the best one (0: all)
 
     @classmethod
     def greedy(cls, max_tokens: int) -> "GenerateParams":
         return cls(max_tokens=max_tokens)
 
     def validate(self) -> None:
-        validate_sampling(self.temperature, self.top_p)
+        validate_sampling(self.temperature, self.top_p, self.top_k, self.min_p)
         if self.max_tokens < 0:
             raise ValueError("max_tokens is negative")
         if any(s == "" for s in self.stop):

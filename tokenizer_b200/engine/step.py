@@ -315,14 +315,14 @@ class Engine:
         self.steps_run += n_steps
         return history
 
-    def sample(self, logits: torch.Tensor, temperature, top_p, uniform) -> List[int]:
+    def sample(self, logits: torch.Tensor, temperature, top_p, uniform, top_k=None, min_p=None) -> List[int]:
         """Draw one id per row of `logits` on the device."""
-        return self.sample_launch(logits, temperature, top_p, uniform).result()
+        return self.sample_launch(logits, temperature, top_p, uniform, top_k, min_p).result()
 
-    def sample_launch(self, logits: torch.Tensor, temperature, top_p, uniform):
+    def sample_launch(self, logits: torch.Tensor, temperature, top_p, uniform, top_k=None, min_p=None):
         """Start the draw; `.result()` of what is returned waits for the ids."""
         with torch.cuda.device(self.runtime.device):
-            return self.sampler.sample_launch(logits, temperature, top_p, uniform)
+            return self.sampler.sample_launch(logits, temperature, top_p, uniform, top_k, min_p)
 
     # ---- a decoding step packed ahead of its tokens --------------------------------
     def prepare_decode(self, caches) -> Optional["PreparedDecode"]:
