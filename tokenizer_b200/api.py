@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import json
 import os
+from dataclasses import replace
 from typing import Callable, List, Optional, Sequence, Union
 
 from .engine.generate import Control, Generated, GenerateParams, StopReason
@@ -14,7 +15,7 @@ from .engine.scheduler import Scheduler
 from .engine.step import Engine, load_model, random_model
 
 __all__ = ["Control", "Engine", "Generated", "GenerateParams", "StopReason", "generate",
-           "generate_batch", "generate_with", "greedy_tokens", "load_eos_token_ids", "load_model",
+           "generate_batch", "generate_samples", "generate_with", "greedy_tokens", "load_eos_token_ids", "load_model",
            "engine_for", "random_model"]
 
 
@@ -37,12 +38,12 @@ def load_eos_token_ids(path: str) -> List[int]:
 
 
 def engine_for(model, tokens: int, page_size: int = 16, max_requests: int = 64,
-               share_prefixes: bool = True) -> Engine:
+               share_prefixes: bool = True, shared_attention: bool = False) -> Engine:
     """An engine whose pool holds `tokens` tokens (rounded up to whole pages
     per request by the caller)."""
     pages = max(1, -(-int(tokens) // page_size))
     return Engine(model, num_pages=pages, page_size=page_size, max_requests=max_requests,
-                  share_prefixes=share_prefixes)
+                  share_prefixes=share_prefixes, shared_attention=shared_attention)
 
 
 def generate_batch(model_or_engine, prompts: Sequence[Sequence[int]],
@@ -72,6 +73,40 @@ def generate_batch(model_or_engine, prompts: Sequence[Sequence[int]],
     for index, (prompt, p) in enumerate(zip(prompts, params)):
         callback = (lambda text, index=index: on_chunk(index, text)) if on_chunk else None
         ids.append(scheduler.add_request(prompt, p, token_bytes, callback))
+    results = scheduler.run()
+    return [results[i] for i in ids]
+
+
+def sample_params(params: Union[GenerateParams, Sequence[GenerateParams]], n: int) -> List[GenerateParams]:
+    """The options of `n` answers to one prompt: one GenerateParams stands for all, answer i with its seed + i."""
+    if isinstance(params, GenerateParams):
+        return [replace(params, seed=params.seed + i) for i in range(n)]
+    if len(params) != n:
+        raise ValueError("one GenerateParams for all answers, or one each")
+    return list(params)
+
+
+def generate_samples(model_or_engine, prompt: Sequence[int], n: int,
+                     params: Union[GenerateParams, Sequence[GenerateParams]],
+                     token_bytes: Optional[Callable[[int], bytes]] = None,
+                     on_chunk: Optional[Callable[[int, str], Control]] = None,
+                     max_batch_size: int = 64, token_budget: int = 2048, page_size: int = 16) -> List[Generated]:
+    """`n` answers to one prompt.  The prompt is computed once; the others are forked from its cache (its full pages shared,
+    the begun one copied) and decode beside it, the common keys read once a step for all of them where that pays.  One
+    GenerateParams stands for all (answer i draws with its seed + i), or one each; `on_chunk(index, text)` may return
+    Control.STOP."""
+    if n < 1:
+        raise ValueError("a prompt is asked for at least one answer")
+    each = sample_params(params, n)
+    if hasattr(model_or_engine, "step") and hasattr(model_or_engine, "cache"):
+        engine = model_or_engine
+    else:
+        batch = max(1, min(max_batch_size, n))
+        own = max((q.max_tokens for q in each), default=0) // page_size + 2       # pages behind the prompt's full ones
+        engine = engine_for(model_or_engine, (len(prompt) // page_size + batch * own) * page_size, page_size, max_requests=batch,
+                            shared_attention=True)
+    scheduler = Scheduler(engine, max_batch_size=min(max_batch_size, engine.cache.max_requests), token_budget=token_budget)
+    ids = scheduler.add_samples(prompt, each, token_bytes, on_chunk)
     results = scheduler.run()
     return [results[i] for i in ids]
 

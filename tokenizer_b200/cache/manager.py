@@ -51,6 +51,7 @@ class RequestCache:
     length: int = 0
     state_slot: int = -1
     closed: bool = False
+    generation: int = 0          # how often its pages have been given back while it was open
     published: object = None     # where publishing the prompt's pages got to (None: not begun; False: broken)
 
     def pages_held(self, group: int) -> List[int]:
@@ -266,6 +267,7 @@ class CachePlan:
                     allocator.give_back(page)
             cache.tables[g] = []
         cache.length = 0
+        cache.generation += 1
         cache.published = None
 
     def close(self, cache: RequestCache) -> None:

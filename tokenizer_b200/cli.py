@@ -11,7 +11,9 @@ be set: --num-pages N (pages of the cache; default: room for every prompt to its
 default 8 as the reference's server: qwen-server/src/lib.rs:47-55), --token-budget N (tokens a
 step may run: prompts are cut into portions under it; default 2048).  --num-blocks,
 --block-size and --prefill-chunk are other names for the first, second and fourth.  With a
-small --num-pages requests are preempted and recomputed; the ids do not change."""
+small --num-pages requests are preempted and recomputed; the ids do not change.  --top-k K and --min-p M filter the
+candidates of a draw beside --top-p; --samples N answers every prompt N times, answer i with the seed plus i, the prompt
+computed once and the others forked from it."""
 from __future__ import annotations
 
 import os
@@ -19,7 +21,7 @@ import sys
 import tempfile
 import time
 
-USAGE = ("usage: qwen-infer [--max-tokens N] [--temperature T] [--top-p P] [--seed N] "
+USAGE = ("usage: qwen-infer [--max-tokens N] [--temperature T] [--top-p P] [--top-k K] [--min-p M] [--seed N] [--samples N] "
          "[--stop STRING]... [--model DIR | --random-weights CONFIG.json] [--dtype bfloat16|float32] "
          "[--num-pages N] [--page-size N] [--max-batch-size N] [--token-budget N] "
          "[--ids 1,2,3]... [<prompt>]...")
@@ -33,7 +35,7 @@ def parse_args(argv):
     args = dict(prompts=[], ids=[], max_tokens=20, temperature=0.0, top_p=1.0, seed=0, stop=[],
                 model=os.environ.get("QWEN_INFER_MODEL"), random_weights=None, dtype="bfloat16",
                 weights_seed=0, device="cuda:0", num_pages=None, page_size=16, max_batch_size=8,
-                token_budget=2048)
+                token_budget=2048, top_k=0, min_p=0.0, samples=1)
     it = iter(argv)
 
     def value(flag):
@@ -51,6 +53,12 @@ def parse_args(argv):
             args["temperature"] = _number(float, value(arg), arg)
         elif arg == "--top-p":
             args["top_p"] = _number(float, value(arg), arg)
+        elif arg == "--top-k":
+            args["top_k"] = _number(int, value(arg), arg)
+        elif arg == "--min-p":
+            args["min_p"] = _number(float, value(arg), arg)
+        elif arg == "--samples":
+            args["samples"] = _positive(value(arg), arg)
         elif arg == "--seed":
             args["seed"] = _number(int, value(arg), arg)
         elif arg == "--stop":
@@ -143,15 +151,17 @@ def main(argv=None) -> int:
     if any(not ids for ids in prompts):
         print("prompt encoded to no tokens", file=sys.stderr)
         return 1
-    several = len(prompts) > 1
+    samples = args["samples"]
+    several = len(prompts) * samples > 1
     for index, ids in enumerate(prompts):
-        label = f"prompt {index} ids" if several else "prompt ids"
+        label = f"prompt {index} ids" if len(prompts) > 1 else "prompt ids"
         print(f"{label} ({len(ids)}): {ids}", file=sys.stderr)
 
     params = tb.GenerateParams(max_tokens=args["max_tokens"], temperature=args["temperature"],
                                top_p=args["top_p"], seed=args["seed"],
-                               eos=tb.load_eos_token_ids(folder), stop=args["stop"])
-    print(f"max_tokens {params.max_tokens} temperature {params.temperature} top_p {params.top_p} "
+                               eos=tb.load_eos_token_ids(folder), stop=args["stop"], top_k=args["top_k"], min_p=args["min_p"])
+    filters = f"top_k {params.top_k} min_p {params.min_p} " if params.top_k or params.min_p else ""
+    print(f"max_tokens {params.max_tokens} temperature {params.temperature} top_p {params.top_p} {filters}"
           f"seed {params.seed} eos {list(params.eos)}", file=sys.stderr)
     scheduler = None
     try:
@@ -160,14 +170,14 @@ def main(argv=None) -> int:
         page = args["page_size"]
         pages = args["num_pages"]
         if pages is None:
-            pages = sum(-(-(len(ids) + params.max_tokens + 1) // page) for ids in prompts)
-        batch = min(args["max_batch_size"], len(prompts))
+            pages = samples * sum(-(-(len(ids) + params.max_tokens + 1) // page) for ids in prompts)
+        batch = min(args["max_batch_size"], len(prompts) * samples)
         engine = tb.Engine(model, num_pages=pages, page_size=page, max_requests=batch,
-                           share_prefixes=True)
+                           share_prefixes=True, shared_attention=samples > 1)
         started = time.perf_counter()
         token_bytes = (lambda t: tokenizer.decode_bytes([t])) if tokenizer else None
         scheduler = tb.Scheduler(engine, max_batch_size=batch, token_budget=args["token_budget"])
-        ids = [scheduler.add_request(p, params, token_bytes) for p in prompts]
+        ids = [i for p in prompts for i in scheduler.add_samples(p, tb.api.sample_params(params, samples), token_bytes)]
         finished = scheduler.run()
         results = [finished[i] for i in ids]
         elapsed = time.perf_counter() - started

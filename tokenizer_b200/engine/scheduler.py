@@ -32,6 +32,10 @@ cursors one by one; ids after a request's end are dropped with its cache.  The
 host's share of a step is paid once a burst.  When the pool has no pages for the
 whole burst the iteration runs a single step as above.
 
+Several answers to one prompt (`add_samples`) are requests of their own of which the first runs the prompt.  When its last
+token has been computed the others are forked from its cache and draw their first ids from the same logits; those that no
+batch slot or page is left for wait in line as any request does, and find the prompt's full pages shared.
+
 The reference's scheduler (qwen-server/src/engine.rs:229-402, 455-704) admits
 and preempts in the same way but runs a whole prompt per iteration; the token
 budget and the portions are this engine's.
@@ -60,6 +64,7 @@ class SchedulerStats:
     tokens_run: int = 0
     tokens_sampled: int = 0
     shared_prefix_tokens: int = 0
+    forked: int = 0
 
 
 @dataclass
@@ -72,14 +77,15 @@ class _Request:
     published: bool = False
     arrived: float = 0.0
     prompt_done: Optional[float] = None
+    forks: List["_Request"] = field(default_factory=list)    # the other answers to its prompt, until it is computed
 
 
 class Scheduler:
     def __init__(self, engine, max_batch_size: int = 8, token_budget: int = 512,
                  decode_burst: int = 1):
         """`engine` offers `cache` (a CachePlan), `step(entries) -> logits`,
-        `sample(logits, temperature, top_p, uniform) -> ids` and
-        `max_positions`; for bursts also `decode_steps(entries, n) -> ids[n][entries]`."""
+        `sample(logits, temperature, top_p, uniform) -> ids` (with `top_k` and `min_p` behind them once a request asks for
+        either) and `max_positions`; for bursts also `decode_steps(entries, n) -> ids[n][entries]`."""
         if max_batch_size < 1 or token_budget < 1:
             raise ValueError("the batch holds at least one request and one token")
         if decode_burst < 1:
@@ -104,18 +110,50 @@ class Scheduler:
     def add_request(self, prompt: Sequence[int], params: GenerateParams,
                     token_bytes: Optional[Callable[[int], bytes]] = None,
                     on_chunk: Optional[Callable[[str], Control]] = None) -> int:
+        return self.add_samples(prompt, [params], token_bytes, None if on_chunk is None else lambda _index, text: on_chunk(text))[0]
+
+    def add_samples(self, prompt: Sequence[int], params: Sequence[GenerateParams],
+                    token_bytes: Optional[Callable[[int], bytes]] = None,
+                    on_chunk: Optional[Callable[[int, str], Control]] = None) -> List[int]:
+        """An answer to `prompt` for each of `params` (each with a seed of its own, or they are alike), the prompt computed
+        once; returns their request ids.  `on_chunk(index, text)` as for `add_request`."""
         prompt = [int(t) for t in prompt]
         if not prompt:
             raise ValueError("the prompt has no tokens")
-        if len(prompt) + params.max_tokens > self.engine.max_positions:
-            raise ValueError(
-                f"prompt of {len(prompt)} plus max_tokens {params.max_tokens} exceeds "
-                f"max_position_embeddings {self.engine.max_positions}")
-        request = _Request(self._next_id, prompt, SampleCursor(params, token_bytes, on_chunk),
-                           list(prompt), arrived=time.perf_counter())
-        self._next_id += 1
-        self.waiting.append(request)
-        return request.id
+        if not params:
+            raise ValueError("a prompt is asked for at least one answer")
+        made = []
+        for index, p in enumerate(params):
+            if len(prompt) + p.max_tokens > self.engine.max_positions:
+                raise ValueError(
+                    f"prompt of {len(prompt)} plus max_tokens {p.max_tokens} exceeds "
+                    f"max_position_embeddings {self.engine.max_positions}")
+            callback = None if on_chunk is None else (lambda text, index=index: on_chunk(index, text))
+            made.append(_Request(self._next_id + index, prompt, SampleCursor(p, token_bytes, callback), list(prompt),
+                                 arrived=time.perf_counter()))
+        self._next_id += len(made)
+        made[0].forks = made[1:]
+        self.waiting.append(made[0])
+        return [r.id for r in made]
+
+    def _fork(self, r: _Request) -> List[_Request]:
+        """The prompt of `r` is computed: fork the other answers to it, as many as there are batch slots and pages for (the
+        others join the line in front of younger requests).  Returns those that now run."""
+        forks, r.forks = r.forks, []
+        n = min(len(forks), self.max_batch_size - len(self.running), self.cache.can_fork(r.cache))
+        for fork, cache in zip(forks, self.cache.fork(r.cache, [f.id for f in forks[:n]])):
+            fork.cache = cache
+            fork.published = True          # the prompt's pages are its parent's
+            fork.prompt_done = r.prompt_done
+            self.running.append(fork)
+        self._wait_in_line(forks[n:])
+        self.stats.forked += n
+        return forks[:n]
+
+    def _wait_in_line(self, requests: List[_Request]) -> None:
+        younger = next((at for at, w in enumerate(self.waiting) if requests and w.id > requests[0].id), len(self.waiting))
+        for at, r in enumerate(requests):
+            self.waiting.insert(younger + at, r)
 
     def has_work(self) -> bool:
         return bool(self.waiting or self.running)
@@ -229,7 +267,7 @@ class Scheduler:
         n = self.decode_burst
         for r in self.running:
             c = r.cursor
-            if len(r.context) - r.cache.length != 1 or c.params.temperature != 0.0 or c.done is not None:
+            if len(r.context) - r.cache.length != 1 or c.params.temperature != 0.0 or c.done is not None or r.forks:
                 return 0
             n = min(n, c.params.max_tokens - c.produced, self.engine.max_positions - len(r.context))
         return n
@@ -345,21 +383,28 @@ class Scheduler:
 
     def _sample(self, ready: List[_Request], logits) -> None:
         now = time.perf_counter()
-        rows, drawing = [], []
+        rows, drawing, computed = [], [], len(ready)
+        forked = []
         for row, r in enumerate(ready):
             if r.prompt_done is None:
                 r.prompt_done = now
             if not r.published and r.cache.length >= len(r.prompt):
                 self.cache.publish_prompt(r.cache, r.prompt)
                 r.published = True
-            if r.cursor.wants_sample():
-                rows.append(row)
-                drawing.append(r)
+            same_row = [r] + (self._fork(r) if r.forks else [])
+            forked += same_row[1:]
+            for request in same_row:
+                if request.cursor.wants_sample():
+                    rows.append(row)
+                    drawing.append(request)
+        ready = ready + forked
         if drawing:
-            picked = logits if len(rows) == len(ready) else logits[rows]
+            picked = logits if rows == list(range(computed)) else logits[rows]
             draw = [picked, [r.cursor.params.temperature for r in drawing],
                     [r.cursor.params.top_p for r in drawing],
                     [r.cursor.next_uniform() for r in drawing]]
+            if any(r.cursor.params.top_k > 0 or r.cursor.params.min_p > 0 for r in drawing):
+                draw += [[r.cursor.params.top_k for r in drawing], [r.cursor.params.min_p for r in drawing]]
             launch = getattr(self.engine, "sample_launch", None)
             if launch is None:
                 ids = self.engine.sample(*draw)
@@ -388,6 +433,8 @@ class Scheduler:
         self.stats.requests_finished += 1
 
     def _fail(self, r: _Request, message: str) -> None:
+        forks, r.forks = r.forks, []
+        self._wait_in_line(forks)              # what it was refused for may not hold for them
         self.finished[r.id] = Generated(list(r.cursor.tokens), r.cursor.text, list(r.cursor.chunks),
                                         StopReason.FAILED, r.cursor.produced, error=message)
         self.stats.requests_failed += 1

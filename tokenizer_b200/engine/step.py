@@ -79,7 +79,10 @@ class PreparedDecode:
 
 class Engine:
     def __init__(self, model: DecoderModel, num_pages: int, page_size: int = 16,
-                 max_requests: int = 64, share_prefixes: bool = False, use_graphs: bool = True):
+                 max_requests: int = 64, share_prefixes: bool = False, use_graphs: bool = True, shared_attention: bool = False):
+        """`shared_attention`: decoding steps whose requests hold the same pages (a shared prompt, forks) read those once for
+        all of them, in every layer that reads all its keys (`ops.shared_prefix_attention`); the sums of its softmax are cut
+        at the end of the common keys, so logits differ in rounding from those of the other kernels."""
         self.model = model
         self.runtime = model.runtime
         self.cache = DeviceCache(model.cache_needs(), num_pages, page_size, max_requests,
@@ -87,6 +90,8 @@ class Engine:
         self.bindings = self.cache.bindings(model.order)
         self.builder = BatchBuilder(self.cache, model.vocab_size, model.max_positions,
                                     model.runtime.device, model.batch_annotations())
+        self.shared_notes = self._shared_notes() if shared_attention else []
+        self.builder.annotations += self.shared_notes
         self.sampler = Sampler(model.runtime.device)
         self.max_positions = model.max_positions
         self.steps_run = 0
@@ -101,6 +106,23 @@ class Engine:
         reach = min(model.max_positions, max(num_pages * page_size, 4096))
         tables = sum(max_requests * (reach // page_size + 8) for _ in self.cache.groups)
         self.builder.reserve_capacity(16 * 8192 + tables)
+
+    def _shared_notes(self):
+        """One annotation a group of keys that attention may read behind common beginnings."""
+        from ..parts.attention import PagedAttention, SharedBeginnings
+        size, notes = torch.empty((), dtype=self.runtime.dtype).element_size(), []
+        for g, layout in enumerate(self.cache.groups):
+            readers = [self.model.blocks[call.layer].mixer for call, binding in zip(self.model.order, self.bindings) if binding.group == g]
+            readers = [m for m in readers if isinstance(m, PagedAttention) and ops.shared_prefix_supported(m.nh, m.nkv, m.d)]
+            if layout.keeps_all and readers:
+                notes.append(SharedBeginnings(g, self.cache.page_size, layout.planes * layout.kv_heads * layout.head_dim * size,
+                                              min(ops.shared_prefix_tile_members(m.nh, m.nkv) for m in readers)))
+        return notes
+
+    def _look(self, entries: List[StepEntry]):
+        """What the annotations about the cache say of a step's requests (part of a captured step's key)."""
+        single = all(len(e.tokens) == 1 for e in entries)
+        return tuple(note.look([e.cache for e in entries], single) for note in self.shared_notes)
 
     @classmethod
     def from_folder(cls, folder: str, dtype="bfloat16", device="cuda:0", **kw) -> "Engine":
@@ -131,6 +153,7 @@ class Engine:
             if shape is not None:
                 logits = self._step_captured(entries, *shape)
             else:
+                self._look(entries)
                 ctx, want_rows, n_want = self.builder.build(entries)
                 logits = self.model.forward(ctx, self.bindings, want_rows[:n_want])
         for e in entries:
@@ -170,8 +193,10 @@ class Engine:
         pages = [max(len(e.cache.tables[g]) for e in entries) for g in range(len(self.cache.groups))]
         longest = max(len(e.tokens) for e in entries)
         if longest == 1:
-            rows = self._bucket(len(entries))
-            return (rows, tuple(self._width(n) for n in pages)), rows, rows
+            rows, common = self._bucket(len(entries)), self._look(entries)
+            key = (rows, tuple(self._width(n) for n in pages))
+            return key if not any(common) else ("common",) + key + (common,), rows, rows
+        self._look(entries)
         # the kernels for portions size their grids from the rows, not from the tables' reach:
         # powers of two keep the shapes of a busy scheduler few
         widths = tuple(self._bucket(n, 8) for n in pages)
@@ -193,13 +218,18 @@ class Engine:
         kinds = self.model.shape_key([len(e.tokens) for e in entries])
         return ("portions", padded, requests, widths, kinds), padded, requests
 
+    @staticmethod
+    def _widths_of(key):
+        """Block-table widths in the key of a step of single tokens."""
+        return key[2] if key[0] == "common" else key[1]
+
     def _step_captured(self, entries: List[StepEntry], key, tokens: int, requests: int) -> torch.Tensor:
         """A step whose launches are captured once per shape (padded batch size,
         padded block-table widths, token count) and replayed afterwards; only the
         packed metadata changes between replays, at fixed addresses.  Idle rows of
         the padded batch carry request -1, which kernels skip."""
         from ..kernels.ops import counter
-        widths = list(key[1] if len(key) == 2 else key[3])
+        widths = list(key[3] if key[0] == "portions" else self._widths_of(key))
         ctx, want_rows, n_want = self.builder.build(
             entries, pad_requests=requests, pad_tokens=tokens, pad_want=requests, table_widths=widths)
         if self._graph_buffer != self.builder.device_buffer_ptr():
@@ -255,12 +285,13 @@ class Engine:
             rows = self._bucket(len(entries))
             widths = [self._width(max(len(e.cache.tables[g]) for e in entries))
                       for g in range(len(self.cache.groups))]
+            common = self._look(entries)
             ctx, want_rows, n_want = self.builder.build(
                 entries, pad_requests=rows, pad_tokens=rows, pad_want=rows, table_widths=widths)
             if self._graph_buffer != self.builder.device_buffer_ptr():
                 self._graphs.clear()
                 self._graph_buffer = self.builder.device_buffer_ptr()
-            key = ("steps", rows, tuple(widths))
+            key = ("steps", rows, tuple(widths), common)
             slot = self._graphs.get(key)
             if slot is None:
                 slot = self._graphs[key] = {
@@ -339,7 +370,7 @@ class Engine:
             return None
         self.builder.validate(entries)
         packed = self.builder.pack(entries, pad_requests=requests, pad_tokens=tokens,
-                                   pad_want=requests, table_widths=list(key[1]))
+                                   pad_want=requests, table_widths=list(self._widths_of(key)))
         return PreparedDecode(entries, key, packed, [c.length for c in caches])
 
     def step_prepared_device(self, prepared: "PreparedDecode", pending) -> Optional[torch.Tensor]:

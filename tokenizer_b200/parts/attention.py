@@ -17,6 +17,7 @@ import os
 import numpy as np
 import torch
 
+from ..cache import sharing
 from ..config.spec import ConfigError
 from ..kernels import ops
 from ..weights.store import TensorSpec
@@ -140,6 +141,69 @@ class RowsByLength(BatchAnnotation):
         return (len(out) - 4) if padded else n
 
 
+class SharedBeginnings(BatchAnnotation):
+    """Of a step of single tokens: which rows' caches begin with the same pages of a group, as
+    `ops.shared_prefix_attention` takes them: int32 [T] common keys a row, [R] members, [R, 4] tiles.  The engine makes one a
+    group of keys that keeps all its pages, if it is asked to (`Engine(shared_attention=True)`).
+
+    Requests keep their sets while they run (pages become common when a request opens or is forked, and stay so until it
+    ends), so the sets are looked for again only when the step's requests change."""
+
+    # Sets that save less reading than this are left to the kernel that reads every row's keys: us a layer, common keys apart / the
+    # decoding kernel, behind what they save: 28 heads over 4 of 128, 8 rows, 15 MB 11.2 / 10.6, 29 MB 12.3 / 13.2; 14 over 2 of 64, 32
+    # rows, 33 MB 11.9 / 12.3, 64 rows, 33 MB 11.2 / 12.6, 68 MB 11.9 / 17.0; 8 over 8 of 64, 16 rows, 31 MB 9.5 / 11.3
+    LEAST_BYTES = 24e6
+
+    def __init__(self, group: int, page_size: int, key_bytes: int, tile_members: int):
+        """`key_bytes`: of one token's row(s) in one call's cache."""
+        self.group, self.page_size, self.key_bytes, self.tile_members = group, page_size, key_bytes, tile_members
+        self.key = f"shared_beginnings_{group}"
+        self._caches, self._plan, self._tiles = [], None, 0
+
+    def look(self, caches, single) -> int:
+        if not single:
+            self._caches, self._plan, self._tiles = [], None, 0
+            return 0
+        if len(caches) != len(self._caches) or \
+                any(a is not b or a.generation != generation for a, (b, generation) in zip(caches, self._caches)):
+            self._caches = [(c, c.generation) for c in caches]
+            self._plan, self._tiles = self._sets(caches), 0
+            if self._plan is not None:
+                self._tiles = 1
+                while self._tiles < len(self._plan[2]):
+                    self._tiles *= 2
+        return self._tiles
+
+    def _sets(self, caches):
+        tables = [c.tables[self.group] for c in caches]
+        usable = [c.length // self.page_size for c in caches]
+        most = max(usable, default=0)
+        if len(caches) < 2 or most == 0:
+            return None
+        table = np.full((len(caches), most), -1, dtype=np.int32)
+        for row, (pages, n) in enumerate(zip(tables, usable)):
+            table[row, :n] = pages[:n]
+        shared, members, tiles = sharing.plan(table, usable, self.page_size, self.tile_members)
+        saved = int(shared.sum(dtype=np.int64)) - int(tiles[:, 2].sum(dtype=np.int64))
+        return (shared, members, tiles) if len(tiles) and saved * self.key_bytes >= self.LEAST_BYTES else None
+
+    def capacity(self, n_tokens, n_requests):
+        return 6 * (-(-n_requests // 4) * 4)
+
+    def fill(self, out, first_rows, counts, starts, padded):
+        if self._plan is None or len(self._plan[0]) != len(counts):
+            return 0
+        n, (shared, members, tiles) = len(out) // 6, self._plan
+        out[:tiles.size] = tiles.reshape(-1)
+        out[4 * n:4 * n + len(shared)] = shared
+        out[5 * n:5 * n + len(members)] = members
+        return self._tiles if padded else len(tiles)
+
+    def view(self, words):
+        n = words.numel() // 6
+        return words[:4 * n].view(-1, 4), words[4 * n:5 * n], words[5 * n:]
+
+
 # the tiles of the two prompt kernels: 64 rows (mma.sync) and 128 rows (tcgen05), for all
 # requests and for those alone that bring more than one token
 _TILES = RowTiles(ops.PREFILL_TILE_ROWS)
@@ -230,6 +294,15 @@ class PagedAttention:
         k_pool = cache.k_pool
         v_pool = cache.v_pool if cache.v_pool is not None else cache.k_pool
         sink = self.sink
+        common = ctx.views.get(f"shared_beginnings_{cache.group}")
+        if common is not None and common[1] > 0 and ctx.max_q_len == 1 and self.window is None and self.chunk is None and \
+                ops.shared_prefix_supported(self.nh, self.nkv, self.d) and \
+                (q.dtype == torch.float32 or ops.shared_prefix_tcgen05_supported(self.nh, self.nkv, self.d, group.page_size)):
+            (tiles, shared, members), n_tiles = common
+            ops.shared_prefix_attention(q, k_pool, v_pool, out, group.block_table, ctx.row_req, ctx.pos, shared[:ctx.n_tokens],
+                                        members, tiles[:n_tiles], self.nh, self.nkv, self.d, group.page_size, self.scale, sink=sink,
+                                        softcap=self.softcap)
+            return
         if q.dtype == torch.bfloat16 and ctx.max_q_len == 1 and \
                 ops.decode_attention_supported(self.nh, self.nkv, self.d):
             rows, even = self._by_length(ctx, group)

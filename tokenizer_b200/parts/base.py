@@ -202,6 +202,11 @@ class BatchAnnotation:
                                   capacities allow.  The count travels with the view.
       view(words) -> Any          the device-side int32 words (a tensor of `capacity`) as the
                                   part wants to see them
+
+    An annotation about what requests hold in the cache (which spans do not say) looks at them itself:
+
+      look(caches, single) -> int the step's requests in order (`RequestCache`), and whether each brings one token; called
+                                  before `fill`.  Returns a number that is part of a captured step's key.
     """
 
     key = ""
