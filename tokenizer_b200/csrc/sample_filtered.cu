@@ -87,22 +87,24 @@ __device__ __forceinline__ unsigned fs_key(float v) {
 __device__ __forceinline__ float fs_value(unsigned key) { return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key); }
 __device__ __forceinline__ u64 fs_order(float v, int id) { return (u64)fs_key(v) << 32 | (unsigned)~id; }
 
-// What a row's weights need: t = (l - max) log2(e) / T, 2^t as 2^(n / 64) from a table times the series of 2^r, |r| <=
-// 1/128, to the fifth power (what is left out is below 2^-55), rounded to a whole number of 2^-S.
+// What a row's weights need: t = (l - max) log2(e) / T, 2^t as 2^(n / 1,024) from a table times the series of 2^r, |r| <=
+// 1 / 2,048, to its square (what is left out is below 2^-37 of a weight, a hundredth of what moves a draw among 150,000 equal
+// candidates), rounded to a whole number of 2^-S.  With a table of 64 and the fifth power, pass 2 of 8 rows of 152,000 took 9.7 us
+// instead of 8.9.
+#define FS_TABLE 1024
 struct FsWeight {
   double max, rate, least, unit;
-  const double* table;      // 2^(j / 64)
+  const double* table;      // 2^(j / FS_TABLE)
   __device__ __forceinline__ double plain(float l) const {
     const double t = ((double)l - max) * rate;
     if (!(t > least)) return 0.0;                 // below half a unit; a NaN (0 times infinity) too
     constexpr double kRound = 6755399441055744.0; // 1.5 * 2^52: adding it rounds to whole numbers
-    constexpr double c1 = 0.69314718055994530942, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4, c5 = c4 * c1 / 5;
-    const double n = fma(t, 64.0, kRound);
+    constexpr double c1 = 0.69314718055994530942, c2 = c1 * c1 / 2;
+    const double n = fma(t, (double)FS_TABLE, kRound);
     const int whole = __double2loint(n);
-    const double r = fma(n - kRound, -1.0 / 64, t);
-    const double p = fma(r, fma(r, fma(r, fma(r, fma(r, c5, c4), c3), c2), c1), 1.0);
-    const double v = table[whole & 63] * p;
-    return __hiloint2double(__double2hiint(v) + (whole >> 6) * (1 << 20), __double2loint(v));
+    const double r = fma(n - kRound, -1.0 / FS_TABLE, t);
+    const double v = table[whole & (FS_TABLE - 1)] * fma(r, fma(r, c2, c1), 1.0);
+    return __hiloint2double(__double2hiint(v) + (whole >> 10) * (1 << 20), __double2loint(v));
   }
   __device__ __forceinline__ u64 whole(double w) const {        // w <= 1, unit <= 2^50
     return (u64)__double_as_longlong(fma(w, unit, 4503599627370496.0)) & ((1ull << 52) - 1);
@@ -123,7 +125,7 @@ struct FsShared {
   uint4 ids[FS_MAX_CLUSTER];         // the first block's: the first id with the largest logit in each block's slice (x)
   ulonglong2 sums[FS_MAX_CLUSTER];   // the first block's: the weights above min-p's border in each block's slice (x)
   u64 scratch[2][2 * FS_WARPS];      // taken in turn, so that one barrier an exchange is enough
-  double table[64];
+  double table[FS_TABLE];
   float of_warps[3][FS_WARPS];
   unsigned listed, mine;
   int first_id;
@@ -221,7 +223,8 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
     for (int i = 0; i < FS_EACH; ++i) sh.count[tid + i * FS_THREADS] = low_word[tid + i * FS_THREADS] = high_word[tid + i * FS_THREADS] = 0;
   };
   clear();
-  if (tid < 64) sh.table[tid] = exp2(tid / 64.0);
+  static_assert(FS_TABLE == FS_THREADS, "a thread an entry");
+  sh.table[tid] = exp2(tid / (double)FS_TABLE);
   if (tid == 0) { sh.listed = 0; sh.mine = 0; sh.first_id = 0x7fffffff; }
   pdl_wait();
   pdl_launch();
@@ -493,23 +496,33 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
   int in_list = 0;
   unsigned n_front = 0, rank_at = 0;
   u64 front = 0, ranked_sum = 0, ranked = 0;     // of a list of few: this thread's candidate, its rank, the running sum there
-  // ranks of the first n candidates in sh.list, weights behind them at FS_FEW
+  // ranks of the first n candidates in sh.list, weights behind them at FS_FEW: four threads a candidate, each compares it with
+  // every fourth (one thread a candidate took 7.4 us for 250)
+  static_assert(FS_THREADS == 4 * FS_FEW, "four threads a candidate");
+  auto ranks_here = [&](int n) { return (tid & 3) == 0 && tid / 4 < n; };
   auto rank_few = [&](int n, unsigned count, u64 sum) {
-    rank_at = count;
-    ranked_sum = sum;
-    ranked = tid < n ? sh.list[tid] : 0;
-    if (tid < n) {
+    ranked = tid / 4 < n ? sh.list[tid / 4] : ~0ull;
+    rank_at = 0;
+    ranked_sum = 0;
+    if (warp * 8 < n) {
 #pragma unroll 4
-      for (int j = 0; j < n; ++j) {
+      for (int j = tid & 3; j < n; j += 4) {
         const u64 other = sh.list[j], w = sh.list[FS_FEW + j];
         if (other >= ranked) { ++rank_at; ranked_sum += w; }
       }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        rank_at += __shfl_xor_sync(0xffffffffu, rank_at, o);
+        ranked_sum += __shfl_xor_sync(0xffffffffu, ranked_sum, o);
+      }
     }
+    rank_at += count;
+    ranked_sum += sum;
   };
   // among n ranked ones behind `count` others (where none reaches the goal: the last one)
   auto first_ranked = [&](int n, unsigned count, const Goal& goal) {
-    const unsigned at = min(block.min(tid < n && goal.reached(rank_at, ranked_sum) ? rank_at : 0xffffffffu), count + n);
-    const ulonglong2 found = block.from(tid < n && rank_at == at, ranked_sum, ranked);
+    const unsigned at = min(block.min(ranks_here(n) && goal.reached(rank_at, ranked_sum) ? rank_at : 0xffffffffu), count + n);
+    const ulonglong2 found = block.from(ranks_here(n) && rank_at == at, ranked_sum, ranked);
     return Found{found.x, found.y};
   };
   // a longer one: cut into 2,048 parts of its order (or of low..high of it, behind `count` candidates of sum `sum`)
