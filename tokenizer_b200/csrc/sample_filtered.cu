@@ -497,7 +497,7 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
   unsigned n_front = 0, rank_at = 0;
   u64 front = 0, ranked_sum = 0, ranked = 0;     // of a list of few: this thread's candidate, its rank, the running sum there
   // ranks of the first n candidates in sh.list, weights behind them at FS_FEW: four threads a candidate, each compares it with
-  // every fourth (one thread a candidate took 7.4 us for 250)
+  // every fourth (one thread a candidate took 7.4 us for 250, this 3.5)
   static_assert(FS_THREADS == 4 * FS_FEW, "four threads a candidate");
   auto ranks_here = [&](int n) { return (tid & 3) == 0 && tid / 4 < n; };
   auto rank_few = [&](int n, unsigned count, u64 sum) {
@@ -613,6 +613,53 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
   unsigned count = 0;                            // in front of what was asked for, and their sum
   u64 sum = 0, kept = 0;                         // the sum of what is kept so far
   Goal k_goal{true, false, 0.0};
+  // A list of up to 64 holds all that can be kept (top-k of the usual sizes): one warp decides, two candidates a lane, without an
+  // exchange with the others (1 row, top-k 20 with top-p and min-p: 19.0 us with them, 16.2 without).
+  auto draw_from_few = [&]() {
+    if (warp != 0) return;
+    const int n = (int)sh.listed;
+    u64 order[2], at_sum[2] = {0, 0};
+    unsigned at_rank[2] = {0, 0};
+    double w[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      order[e] = lane + 32 * e < n ? sh.list[lane + 32 * e] : ~0ull;
+      w[e] = lane + 32 * e < n ? weight.plain(fs_value((unsigned)(order[e] >> 32))) : 0.0;
+      if (lane + 32 * e < n) sh.list[FS_FEW + lane + 32 * e] = weight.whole(w[e]);
+    }
+    __syncwarp();
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const u64 other = sh.list[j], whole = sh.list[FS_FEW + j];
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (other >= order[e]) { ++at_rank[e]; at_sum[e] += whole; }
+    }
+    auto first = [&](const Goal& goal) {
+      unsigned at = n;                             // none reaches it: the last one
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (lane + 32 * e < n && goal.reached(at_rank[e], at_sum[e])) at = min(at, at_rank[e]);
+      at = __reduce_min_sync(0xffffffffu, at);
+      const unsigned in0 = __ballot_sync(0xffffffffu, lane < n && at_rank[0] == at);
+      const unsigned in1 = __ballot_sync(0xffffffffu, lane + 32 < n && at_rank[1] == at);
+      const int from = __ffs(in0 ? in0 : in1) - 1;
+      return Found{__shfl_sync(0xffffffffu, in0 ? at_sum[0] : at_sum[1], from), __shfl_sync(0xffffffffu, in0 ? order[0] : order[1], from)};
+    };
+    if (by_k) kept = first(k_goal).sum;
+    if (by_p) kept = min(kept, first(Goal{false, false, p_share * (double)kept}).sum);
+    if (by_m) {
+      u64 m_sum = 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (lane + 32 * e < n && w[e] >= m_border) m_sum += weight.whole(w[e]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m_sum += __shfl_xor_sync(0xffffffffu, m_sum, o);
+      kept = min(kept, m_sum);
+    }
+    const Found drawn = first(Goal{false, true, u * (double)kept});
+    if (lane == 0) out[row] = (int)~(unsigned)drawn.order;
+  };
   FsCommand c{};
   c.what = count_only ? FS_COUNTS : FS_SUMS;
   c.is_first = 1;
@@ -646,6 +693,9 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
         });
         listed = at_place(count_to, end) <= FS_LIST;
       }
+    } else if (listed && sh.listed <= 64) {
+      draw_from_few();
+      return;
     } else {
       open_list(count, sum);
       open = true;
@@ -728,9 +778,9 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
 
 // Blocks a cluster.  A block has a multiprocessor to itself, and the device holds some 16 clusters of 8 or 34 of 4 at once: few
 // rows are cut into 8 slices, many into 2.  Slices below some 3,000 logits are not worth an exchange.  us for 8 / 4 / 2 / 1
-// blocks, rows with settings of their own: 152,064 logits, 8 rows 46 / 57 / 94 / 160, 24 58 / 57 / 88 / 141, 64 117 / 97 / 131 / 217; 49,999, 8
-// rows 36 / 37 / 46 / 71, 37 65 / 54 / 63 / 97, 64 88 / 58 / 62 / 98 (from a nucleus 108 / 64 / 43 / 63); 10,007, 37 rows 57 / 40 / 40 / 42; 2,000,
-// 8 rows 23 / 22 / 21 / 21.
+// blocks, rows with settings of their own: 152,064 logits, 8 rows 39 / 53 / 89 / 151, 24 50 / 50 / 78 / 127, 64 103 / 91 / 124 / 206 (all
+// from a nucleus 134 / 98 / 82 / 131); 49,999, 8 rows 31 / 35 / 43 / 66, 37 56 / 48 / 58 / 88, 64 77 / 52 / 58 / 89 (from a nucleus 93 / 57 /
+// 38 / 56); 10,007, 37 rows 48 / 36 / 37 / 36; 2,000, 8 rows 20 / 19 / 19 / 18.
 static int fs_cluster(int n_rows, int vocab) {
   const int by_rows = n_rows <= 15 ? 8 : n_rows <= (vocab > 100000 ? 68 : 34) ? 4 : 2;
   const int by_slice = vocab > 24576 ? 8 : vocab > 8192 ? 4 : vocab > 3000 ? 2 : 1;
