@@ -476,7 +476,7 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: Opti
 def _flat_pairs(pairs):
     """(source, destination, rows) triples as one array of 32-bit integers."""
     try:
-        flat = array.array("i", itertools.chain.from_iterable(pairs))
+        flat = array.array("i", list(itertools.chain.from_iterable(pairs)))
         whole = set(map(len, pairs)) <= {3}
     except (TypeError, OverflowError):
         whole = False
@@ -606,65 +606,71 @@ def shared_prefix_attention(q, k_pool, v_pool, out, block_table, row_req, pos, s
     `shared_prefix_tile_members` of them (a larger set is several tiles; a tile without members is skipped); `members`
     (int32) are rows of the batch, each in one tile at most (-1: none); `shared` (int32, one a row) repeats the tile's
     `keys`, 0 for a row of no tile.  The common keys are read through the block table of the tile's first member.  A row
-    then sees its own keys from `shared` up to its position, so `shared` is at most the position + 1; `shared_prefix_plan`
+    then sees its own keys from `shared` up to its position, so `shared` is at most the position + 1; `cache.sharing.plan`
     makes the three from block tables.  Rows of request -1 are left as they are.  `sink` and `softcap` as in the other
     attention kernels; `block_table`, `row_req`, `pos` as theirs."""
-    rows = q.shape[0]
-    if q.dtype not in _DTYPE_TAG or k_pool.dtype != q.dtype or v_pool.dtype != q.dtype or out.dtype != q.dtype:
-        raise ValueError("shared_prefix_attention: q, keys, values and out are all float32 or all bfloat16")
+    what, rows, dtype = "shared_prefix_attention", q.shape[0], q.dtype
+    if dtype not in _DTYPE_TAG or k_pool.dtype != dtype or v_pool.dtype != dtype or out.dtype != dtype:
+        raise ValueError(f"{what}: q, keys, values and out are all float32 or all bfloat16")
     if nkv < 1 or not shared_prefix_supported(nh, nkv, d):
-        raise ValueError(f"shared_prefix_attention: {nh} heads over {nkv} groups of size {d} is not taken")
-    if q.numel() != rows * nh * d or out.shape != q.shape or k_pool.shape != v_pool.shape or k_pool.numel() % (nkv * d):
-        raise ValueError("shared_prefix_attention: q and out are [rows, heads * size], the pools [slots, kv heads, size]")
-    if page < 1 or block_table.dim() != 2:
-        raise ValueError("shared_prefix_attention: a block table is [requests, pages]")
-    for t, name in ((block_table, "block_table"), (row_req, "row_req"), (pos, "pos"), (shared, "shared"), (members, "members"),
-                    (tiles, "tiles")):
-        if t.dtype != torch.int32:
-            raise ValueError(f"shared_prefix_attention: {name} is int32")
+        raise ValueError(f"{what}: {nh} heads over {nkv} groups of size {d} is not taken")
+    slots, rest = divmod(k_pool.numel(), nkv * d)
+    if q.numel() != rows * nh * d or out.shape != q.shape or k_pool.shape != v_pool.shape or rest or slots >= 1 << 31:
+        raise ValueError(f"{what}: q and out are [rows, heads * size], the pools [slots, kv heads, size]")
+    if page < 1 or block_table.dim() != 2 or block_table.shape[1] < 1:
+        raise ValueError(f"{what}: a block table is [requests, pages]")
+    if not block_table.dtype == row_req.dtype == pos.dtype == shared.dtype == members.dtype == tiles.dtype == torch.int32:
+        raise ValueError(f"{what}: tables, requests, positions and the plan are int32")
     if row_req.numel() != rows or pos.numel() != rows or shared.numel() != rows or tiles.dim() != 2 or tiles.shape[1] != 4:
-        raise ValueError("shared_prefix_attention: row_req, pos and shared have one entry a row, tiles are [n, 4]")
+        raise ValueError(f"{what}: row_req, pos and shared have one entry a row, tiles are [n, 4]")
     if softcap is not None and not softcap > 0:
-        raise ValueError("shared_prefix_attention: a cap on the scores is positive")
-    _here("shared_prefix_attention", q, k_pool, v_pool, out, block_table, row_req, pos, shared, members, tiles, sink)
-    if rows == 0 or block_table.shape[1] == 0:
+        raise ValueError(f"{what}: a cap on the scores is positive")
+    _here(what, q, k_pool, v_pool, out, block_table, row_req, pos, shared, members, tiles, sink)
+    if not (q.is_contiguous() and k_pool.is_contiguous() and v_pool.is_contiguous() and out.is_contiguous() and block_table.is_contiguous() and
+            row_req.is_contiguous() and pos.is_contiguous() and shared.is_contiguous() and members.is_contiguous() and tiles.is_contiguous()):
+        raise ValueError(f"{what}: kernels take contiguous tensors")
+    q_at, k_at, v_at, out_at, shared_at = q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), shared.data_ptr()
+    table_at, req_at, pos_at, members_at, tiles_at = block_table.data_ptr(), row_req.data_ptr(), pos.data_ptr(), members.data_ptr(), tiles.data_ptr()
+    sink_at, cap, stream = _sink(sink, nh).value or 0, float(softcap or 0.0), _stream().value or 0
+    if rows == 0:
         return
-    n_tiles, reach = tiles.shape[0], block_table.shape[1] * page
+    n_tiles, width = tiles.shape[0], block_table.shape[1]
+    reach = width * page
     # the parts are of this launch alone: captured graphs and streams share nothing
-    if q.dtype == torch.bfloat16 and shared_prefix_tcgen05_supported(nh, nkv, d, page) and \
-            (q.data_ptr() | k_pool.data_ptr() | v_pool.data_ptr() | out.data_ptr()) % 16 == 0:
+    if dtype == torch.bfloat16 and shared_prefix_tcgen05_supported(nh, nkv, d, page) and (q_at | k_at | v_at | out_at) % 16 == 0:
         # Rows that have little to read altogether read all of it themselves, in one kernel (us, that / common keys apart, behind
         # 14 heads over 2 of 64: 4 rows of 576 keys 5.0 / 10.1, 16 of 1,152 7.5 / 10.3, 64 of 640 (21 MB) 9.4 / 11.9, of 1,152 (38 MB)
         # 12.0 / 11.2; 28 over 4 of 128: 8 of 640 9.4 / 11.4, 32 of 384 (25 MB) 12.0 / 12.7, 16 of 1,152 15.3 / 11.2; few rows of long
         # reach have too few blocks: 2 of 2,176 11.6 / 11.6, of 4,224 16.0 / 13.0).
         if rows * reach * nkv * d * 4 <= 24e6 and reach * d <= 300000:
-            n_tiles, shared = 0, None
-        lib, tile_pieces, own_pieces = _shared_prefix_plan(d, rows, n_tiles, nkv, reach)
-        parts = rows * nh * tile_pieces if n_tiles else 0
-        scratch = torch.empty(parts * (d + 2), dtype=torch.float32, device=q.device)
-        _check(lib.tokb200_shared_prefix_tcgen05(
-            _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(out), _ptr(block_table), _i(block_table.shape[1]), _ptr(row_req), _ptr(pos),
-            _ptr(shared), _ptr(members), _ptr(tiles), _i(n_tiles), _i(rows), _i(k_pool.numel() // (nkv * d)), _i(nh), _i(nkv), _i(d),
-            _i(page), _f(scale), _sink(sink, nh), _f(softcap or 0.0), _i(tile_pieces), _i(own_pieces), _ptr(scratch), _stream()),
-            "shared_prefix_attention")
+            n_tiles, shared_at = 0, 0
+        launch, tile_pieces, own_pieces = _shared_prefix_plan(d, rows, n_tiles, nkv, reach)
+        scratch = torch.empty(rows * nh * tile_pieces * (d + 2), dtype=torch.float32, device=q.device) if n_tiles else None
+        _check(launch(q_at, k_at, v_at, out_at, table_at, width, req_at, pos_at, shared_at, members_at, tiles_at, n_tiles, rows, slots,
+                      nh, nkv, d, page, scale, sink_at, cap, tile_pieces, own_pieces, 0 if scratch is None else scratch.data_ptr(), stream), what)
         return
-    lib, tile_pieces, own_pieces = _shared_prefix_plan(0, rows, n_tiles, nkv, reach)
+    launch, tile_pieces, own_pieces = _shared_prefix_plan(0, rows, n_tiles, nkv, reach)
     scratch = torch.empty(rows * nh * (tile_pieces + own_pieces) * (d + 2), dtype=torch.float32, device=q.device)
-    _check(lib.tokb200_shared_prefix_attention(
-        _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(out), _i(_tag(q)), _ptr(block_table), _i(block_table.shape[1]), _ptr(row_req),
-        _ptr(pos), _ptr(shared), _ptr(members), _ptr(tiles), _i(n_tiles), _i(shared_prefix_tile_members(nh, nkv)), _i(rows), _i(nh),
-        _i(nkv), _i(d), _i(page), _f(scale), _sink(sink, nh), _f(softcap or 0.0), _i(tile_pieces), _i(own_pieces), _ptr(scratch),
-        _stream()), "shared_prefix_attention")
+    _check(launch(q_at, k_at, v_at, out_at, _tag(q), table_at, width, req_at, pos_at, shared_at, members_at, tiles_at, n_tiles,
+                  shared_prefix_tile_members(nh, nkv), rows, nh, nkv, d, page, scale, sink_at, cap, tile_pieces, own_pieces,
+                  scratch.data_ptr(), stream), what)
 
 
 @functools.lru_cache(maxsize=4096)
 def _shared_prefix_plan(d: int, rows: int, n_tiles: int, nkv: int, reach: int):
-    """(library, pieces of a tile's keys, pieces of a row's own keys) of a launch; d 0: the general kernels."""
-    lib = _load("shared_prefix_tcgen05.cu", defines=(f"HEAD_DIM={d}",)) if d else _lib("shared_prefix")
-    tile_pieces, own_pieces = ctypes.c_int(1), ctypes.c_int(1)
-    plan = lib.tokb200_shared_prefix_tcgen05_pieces if d else lib.tokb200_shared_prefix_pieces
+    """(launcher, pieces of a tile's keys, pieces of a row's own keys) of a launch; d 0: the general kernels."""
+    at, n, f = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+    if d:
+        lib = _load("shared_prefix_tcgen05.cu", defines=(f"HEAD_DIM={d}",))
+        launch, plan = lib.tokb200_shared_prefix_tcgen05, lib.tokb200_shared_prefix_tcgen05_pieces
+        launch.argtypes = [at] * 5 + [n] + [at] * 5 + [n] * 7 + [f, at, f, n, n, at, at]
+    else:
+        lib = _lib("shared_prefix")
+        launch, plan = lib.tokb200_shared_prefix_attention, lib.tokb200_shared_prefix_pieces
+        launch.argtypes = [at] * 4 + [n, at, n] + [at] * 5 + [n] * 7 + [f, at, f, n, n, at, at]
+    tile_pieces, own_pieces = n(1), n(1)
     plan(_i(rows), _i(n_tiles), _i(nkv), _i(reach), ctypes.byref(tile_pieces), ctypes.byref(own_pieces))
-    return lib, tile_pieces.value, own_pieces.value
+    return launch, tile_pieces.value, own_pieces.value
 
 
 _stream_plans = {}
