@@ -20,8 +20,10 @@ DESIGNS = [(m, n) for m, names in [("tiny", "abc"), ("tiny_pufuzen", "pqrst"), (
 @pytest.fixture
 def every_set(monkeypatch):
     """Common keys are read apart however little that saves."""
+    from tokenizer_b200.kernels import ops
     from tokenizer_b200.parts.attention import SharedBeginnings
     monkeypatch.setattr(SharedBeginnings, "LEAST_BYTES", 0)
+    monkeypatch.setattr(ops, "SHARED_PREFIX_LITTLE", 0)
 
 
 @pytest.fixture

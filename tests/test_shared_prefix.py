@@ -28,6 +28,9 @@ def test_sets_of_common_beginnings():
     rows = [[9, 9, 9, 9, 1], [9, 9, 9, 9, 1], [9, 9, 9, 9, 2], [9, 9, 9, 9, 2]]
     assert found(rows) == [([0, 1, 2, 3], 4)]
     assert found([[1, 2], [1, 3]], least=2) == [] and found([[1, 2], [1, 2]], least=2) == [([0, 1], 2)]
+    # nothing behind a hole or behind the table is shared
+    assert found([[1, -1, 3], [1, -1, 3]]) == [([0, 1], 1)] and found([[-1], [-1]]) == []
+    assert found([[1, 2], [1, 2]], [9, 9]) == [([0, 1], 2)]
     # beginnings too short to count do not hide longer ones of parts
     assert found([[1, 2, 3], [1, 2, 3], [1, 4, 5]], least=3) == [([0, 1], 3)]
 
@@ -42,6 +45,13 @@ def test_the_plan_cuts_sets_into_tiles():
     assert tiles.shape == (0, 4) and members.size == 0 and not shared.any()
     with pytest.raises(ValueError):
         sharing.plan(table_of(rows), [1] * 8, 16, 0)
+
+
+@pytest.fixture(params=["apart", "by size"])
+def form(request, monkeypatch):
+    """Common keys read apart however little there is to read, and as the rule on sizes has it."""
+    if request.param == "apart":
+        monkeypatch.setattr(ops, "SHARED_PREFIX_LITTLE", 0)
 
 
 # ---- the attention -----------------------------------------------------------------------------------------------------
@@ -130,7 +140,7 @@ HEADS = [(14, 2, 64, 16), (12, 2, 128, 16), (28, 4, 128, 8), (8, 8, 64, 32), (16
 @pytest.mark.parametrize("nh, nkv, d, page", HEADS)
 @pytest.mark.parametrize("sets, alone, own", [([(4, 3)], 0, [5, 1, 40]), ([(2, 1), (3, 20), (5, 9)], 3, [1, 33, 130, 64]), ([(41, 6)], 1, [17, 3]),
                                               ([], 3, [1, 70])])
-def test_against_the_definition(nh, nkv, d, page, sets, alone, own, dtype):
+def test_against_the_definition(nh, nkv, d, page, sets, alone, own, dtype, form):
     b = make(nh, nkv, d, page, sets, alone, own, dtype, seed=d + page, sink=alone == 1)
     near(run(b, 1 / math.sqrt(d)), plain(b, 1 / math.sqrt(d)), b)
 
@@ -139,17 +149,24 @@ def test_against_the_definition(nh, nkv, d, page, sets, alone, own, dtype):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("keys_pages, own", [(64, [1]), (130, [200, 7]), (1, [1500]), (257, [300])])
 @pytest.mark.parametrize("softcap", [None, 2.5])
-def test_long_beginnings(keys_pages, own, softcap, dtype):
+def test_long_beginnings(keys_pages, own, softcap, dtype, form):
     b = make(14, 2, 64, 16, [(9, keys_pages)], 2, own, dtype, seed=keys_pages, sink=softcap is not None)
     near(run(b, 0.125, softcap), plain(b, 0.125, softcap), b)
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_idle_rows_padded_tiles_and_garbage_behind_the_last_key(dtype):
-    b = make(14, 2, 64, 16, [(6, 5)], 2, [3, 20], dtype, idle=(1, 4))
-    b["members"] = [r for r in b["members"] if b["row_req"][r] >= 0]
-    b["tiles"][0][1] = len(b["members"])
+@pytest.mark.parametrize("listed", [False, True])
+def test_idle_rows_padded_tiles_and_garbage_behind_the_last_key(listed, dtype, form):
+    """Idle rows among the members (the first one too), as -1, or not at all."""
+    b = make(14, 2, 64, 16, [(600, 5)] if listed else [(6, 5)], 2, [3, 20], dtype, idle=(0, 1, 4))
+    if listed:
+        first = b["tiles"][0][0]
+        b["row_req"][b["members"][first]] = -1
+        b["members"][first + 1] = -1 if b["row_req"][b["members"][first + 1]] < 0 else b["members"][first + 1]
+    else:
+        b["members"] = [r for r in b["members"] if b["row_req"][r] >= 0]
+        b["tiles"][0][1] = len(b["members"])
     want = plain(b, 0.125)
     # everything that no row sees: NaN in keys, infinities in values
     seen = torch.zeros(b["k"].shape[0], dtype=torch.bool)
@@ -158,12 +175,12 @@ def test_idle_rows_padded_tiles_and_garbage_behind_the_last_key(dtype):
             seen[[int(b["table"][r, i // 16]) * 16 + i % 16 for i in range(p + 1)]] = True
     b["k"][~seen] = float("nan")
     b["v"][~seen] = float("inf")
-    near(run(b, 0.125, n_pad_tiles=5), want, b)
+    near(run(b, 0.125, n_pad_tiles=0 if listed else 5), want, b)
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_rows_whose_own_keys_are_none(dtype):
+def test_rows_whose_own_keys_are_none(dtype, form):
     """A position at the end of the common keys: the row sees the tile's keys alone; a row that sees nothing is zero."""
     b = make(14, 2, 64, 16, [(5, 4)], 1, [16], dtype)
     for r in range(6):
@@ -179,7 +196,7 @@ def test_rows_whose_own_keys_are_none(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_large_scores_and_repeats(dtype):
+def test_large_scores_and_repeats(dtype, form):
     """Scores far apart (one key holds all the weight), and the same bits every time, alone and in a graph beside another stream."""
     b = make(12, 2, 128, 16, [(20, 40)], 3, [90, 5], dtype)
     b["q"] *= 6
@@ -191,7 +208,7 @@ def test_large_scores_and_repeats(dtype):
 
 
 @pytest.mark.gpu
-def test_captured_graphs_on_two_streams():
+def test_captured_graphs_on_two_streams(form):
     b = make(14, 2, 64, 16, [(9, 33)], 2, [40, 300], torch.bfloat16)
     c = make(14, 2, 64, 16, [(9, 30)], 2, [70, 20], torch.bfloat16, seed=3)
     ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731

@@ -9,10 +9,11 @@ import numpy as np
 
 def common_beginnings(table: np.ndarray, usable: Sequence[int], least: int = 1) -> List[Tuple[List[int], int]]:
     """[(rows, pages)] of disjoint sets of at least two rows whose first `pages` table entries are the same.  `table` is
-    [rows, pages], of row r the first usable[r] entries may be shared.  Where a set's parts have more in common than the
+    [rows, pages], of row r the first usable[r] entries may be shared (none from a hole, -1, on).  Where a set's parts have more in common than the
     whole, it is taken whole or in parts by how many page reads that saves: (rows - 1) * pages.  Sets with fewer than
     `least` pages are left out."""
-    usable = np.asarray(usable, dtype=np.int64)
+    holes = np.concatenate([np.asarray(table) < 0, np.ones((len(table), 1), dtype=bool)], axis=1)
+    usable = np.minimum(np.asarray(usable, dtype=np.int64), holes.argmax(axis=1)) if len(table) else np.zeros(0, dtype=np.int64)
 
     def split(rows, at):
         """`rows` by their entry at place `at`, those that have one."""

@@ -50,7 +50,10 @@ struct __align__(16) FsStats { float max, min; int odd, unused; };       // odd:
 
 __device__ __forceinline__ unsigned fs_rank() { unsigned r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ unsigned fs_size() { unsigned r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ void fs_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fs_arrive() {
+  __syncwarp();                      // the barrier wants a warp whole, whatever loop it comes from
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void fs_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fs_sync() { fs_arrive(); fs_wait(); }
 __device__ __forceinline__ unsigned fs_peer(const void* local, unsigned rank) {

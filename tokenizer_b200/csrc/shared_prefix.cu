@@ -1,7 +1,7 @@
 // Attention of decoding rows whose caches begin with the same pages: the general kernels (any type, head size to 256 and
 // page size; the tensor-core ones for bfloat16 are in shared_prefix_tcgen05.cu).
 //
-// A row r sees the `keys` keys of its tile, read through the table of the tile's first member, and its own keys from
+// A row r sees the `keys` keys of its tile, read through the table of the tile's first live member, and its own keys from
 // shared[r] up to pos[r]; a row of no tile has shared[r] = 0 and sees its own alone.  With scores s = q.k * scale (capped:
 // cap * tanh(s / cap)) the output is sum(exp(s) v) / (sum(exp(s)) + exp(sink)).  A softmax splits along its keys: a part with
 // maximum m, sum l = sum(exp(s - m)) and weighted values a = sum(exp(s - m) v) joins others by sum(exp(m - M) a) / sum(exp(m -
@@ -34,6 +34,16 @@ __device__ __forceinline__ float sp_warp_max(float v) {      // one instruction;
   return m;
 }
 
+// the request whose table a tile's keys are read through: its first live member's (-1: it has none)
+__device__ __forceinline__ int sp_tile_request(const int4& tile, const int* __restrict__ members, const int* __restrict__ row_req) {
+  int req = -1;
+  for (int i = 0; i < tile.y && req < 0; ++i) {
+    const int row = members[tile.x + i];
+    req = row < 0 ? -1 : row_req[row];
+  }
+  return req;
+}
+
 // parts: [row][head][tile_pieces + own_pieces][d + 2]
 template <typename T, int DI>
 __global__ void __launch_bounds__(SP_THREADS, DI <= 4 ? 2 : 1)
@@ -61,10 +71,9 @@ shared_prefix_parts_kernel(const T* __restrict__ q, const T* __restrict__ k_pool
   const int row_alone = common ? -1 : unit;
   if (common) {
     const int4 tile = tiles[unit];
-    const int lead = tile.y > 0 ? members[tile.x] : -1;
     first_member = tile.x;
     n_pairs = tile.y * group;
-    req = lead < 0 ? -1 : row_req[lead];
+    req = sp_tile_request(tile, members, row_req);
     const int keys = min(tile.z, table_stride * page), len = sp_piece(keys, tile_pieces);
     first = piece * len;
     end = min(keys, first + len);

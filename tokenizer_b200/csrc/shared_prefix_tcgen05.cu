@@ -54,6 +54,16 @@ __host__ __device__ __forceinline__ int sp_piece(int n, int pieces) {
   return len < SP_KEYS ? SP_KEYS : len;
 }
 
+// the request whose table a tile's keys are read through: its first live member's (-1: it has none)
+__device__ __forceinline__ int sp_tile_request(const int4& tile, const int* __restrict__ members, const int* __restrict__ row_req) {
+  int req = -1;
+  for (int i = 0; i < tile.y && req < 0; ++i) {
+    const int row = members[tile.x + i];
+    req = row < 0 ? -1 : row_req[row];
+  }
+  return req;
+}
+
 // acc_parts: [row][head][pieces][HEAD_DIM]; stat_parts: [row][head][pieces] (maximum in log2 units, sum)
 template <bool CAPPED>
 __global__ void __launch_bounds__(SP_THREADS, 1)
@@ -102,8 +112,7 @@ shared_prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __
   pdl_wait();
   pdl_launch();
   const int4 tile = tiles[blockIdx.z];
-  const int lead = tile.y > 0 ? members[tile.x] : -1;
-  const int req = lead < 0 ? -1 : row_req[lead];
+  const int req = sp_tile_request(tile, members, row_req);
   const bool aligned = (fa_smem(fa_raw) & 1023u) == 0;
   if (!aligned && threadIdx.x == 0) {
     atomicExch(&sp_error_flag, 2);
@@ -453,6 +462,7 @@ __device__ __forceinline__ unsigned own_pack(float lo, float hi) {
   return *reinterpret_cast<unsigned*>(&v);
 }
 __device__ __forceinline__ void own_cluster_sync() {
+  __syncwarp();                                      // the barrier wants a warp whole, whatever loop it comes from
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 // four floats of block `rank` of this cluster, at the place `local` has in this block's shared memory (no memory clobber: several

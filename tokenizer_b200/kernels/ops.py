@@ -583,6 +583,13 @@ def decode_attention(q, k_pool, v_pool, out, block_table, row_req, pos, nh, nkv,
         _ptr(counters), _ptr(rows), _ptr(even), _sink(sink, nh), _f(softcap or 0.0), _stream()), "decode_attention")
 
 
+# Rows that have no more bytes than this to read altogether read all of it themselves, in one kernel (us, that / common keys apart:
+# 14 heads over 2 of 64, 4 rows of 576 keys 5.0 / 10.1, 16 of 1,152 7.5 / 10.3, 64 of 640 (21 MB) 9.4 / 11.9, of 1,152 (38 MB) 12.0 /
+# 11.2; 28 over 4 of 128, 8 of 640 9.4 / 11.4, 32 of 384 (25 MB) 12.0 / 12.7, 16 of 1,152 (38 MB) 15.3 / 11.2); not few rows of long
+# reach, which have too few blocks (12 over 2 of 128, 2 of 2,176 11.3 / 11.2, of 4,224 15.8 / 12.1).
+SHARED_PREFIX_LITTLE = 24e6
+
+
 def shared_prefix_tile_members(nh: int, nkv: int) -> int:
     """The most members of a tile of `shared_prefix_attention`: their heads of one group fill 256 rows."""
     return max(1, 2 * (128 // (nh // nkv)))
@@ -605,7 +612,7 @@ def shared_prefix_attention(q, k_pool, v_pool, out, block_table, row_req, pos, s
     `tiles` is int32 [n, 4]: (first place in `members`, members, keys, unused) of rows that share their first `keys` keys, at most
     `shared_prefix_tile_members` of them (a larger set is several tiles; a tile without members is skipped); `members`
     (int32) are rows of the batch, each in one tile at most (-1: none); `shared` (int32, one a row) repeats the tile's
-    `keys`, 0 for a row of no tile.  The common keys are read through the block table of the tile's first member.  A row
+    `keys`, 0 for a row of no tile.  The common keys are read through the block table of the tile's first live member.  A row
     then sees its own keys from `shared` up to its position, so `shared` is at most the position + 1; `cache.sharing.plan`
     makes the three from block tables.  Rows of request -1 are left as they are.  `sink` and `softcap` as in the other
     attention kernels; `block_table`, `row_req`, `pos` as theirs."""
@@ -638,11 +645,7 @@ def shared_prefix_attention(q, k_pool, v_pool, out, block_table, row_req, pos, s
     reach = width * page
     # the parts are of this launch alone: captured graphs and streams share nothing
     if dtype == torch.bfloat16 and shared_prefix_tcgen05_supported(nh, nkv, d, page) and (q_at | k_at | v_at | out_at) % 16 == 0:
-        # Rows that have little to read altogether read all of it themselves, in one kernel (us, that / common keys apart, behind
-        # 14 heads over 2 of 64: 4 rows of 576 keys 5.0 / 10.1, 16 of 1,152 7.5 / 10.3, 64 of 640 (21 MB) 9.4 / 11.9, of 1,152 (38 MB)
-        # 12.0 / 11.2; 28 over 4 of 128: 8 of 640 9.4 / 11.4, 32 of 384 (25 MB) 12.0 / 12.7, 16 of 1,152 15.3 / 11.2; few rows of long
-        # reach have too few blocks: 2 of 2,176 11.6 / 11.6, of 4,224 16.0 / 13.0).
-        if rows * reach * nkv * d * 4 <= 24e6 and reach * d <= 300000:
+        if rows * reach * nkv * d * 4 <= SHARED_PREFIX_LITTLE and reach * d <= 300000:
             n_tiles, shared_at = 0, 0
         launch, tile_pieces, own_pieces = _shared_prefix_plan(d, rows, n_tiles, nkv, reach)
         scratch = torch.empty(rows * nh * tile_pieces * (d + 2), dtype=torch.float32, device=q.device) if n_tiles else None
