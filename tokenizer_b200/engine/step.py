@@ -116,7 +116,8 @@ class Engine:
             readers = [m for m in readers if isinstance(m, PagedAttention) and ops.shared_prefix_supported(m.nh, m.nkv, m.d)]
             if layout.keeps_all and readers:
                 notes.append(SharedBeginnings(g, self.cache.page_size, layout.planes * layout.kv_heads * layout.head_dim * size,
-                                              min(ops.shared_prefix_tile_members(m.nh, m.nkv) for m in readers)))
+                                              min(ops.shared_prefix_tile_members(m.nh, m.nkv) for m in readers),
+                                              0 if self.runtime.dtype == torch.float32 else SharedBeginnings.LEAST_BYTES))
         return notes
 
     def _look(self, entries: List[StepEntry]):

@@ -149,14 +149,16 @@ class SharedBeginnings(BatchAnnotation):
     Requests keep their sets while they run (pages become common when a request opens or is forked, and stay so until it
     ends), so the sets are looked for again only when the step's requests change."""
 
-    # Sets that save less reading than this are left to the kernel that reads every row's keys: us a layer, common keys apart / the
-    # decoding kernel, behind what they save: 28 heads over 4 of 128, 8 rows, 15 MB 11.2 / 10.6, 29 MB 12.3 / 13.2; 14 over 2 of 64, 32
-    # rows, 33 MB 11.9 / 12.3, 64 rows, 33 MB 11.2 / 12.6, 68 MB 11.9 / 17.0; 8 over 8 of 64, 16 rows, 31 MB 9.5 / 11.3
+    # In bfloat16, sets that save less reading than this are left to the decoding kernel: us a layer, common keys apart / that kernel,
+    # behind what they save: 28 heads over 4 of 128, 8 rows, 15 MB 11.2 / 10.6, 29 MB 12.3 / 13.2; 14 over 2 of 64, 32
+    # rows, 33 MB 11.9 / 12.3, 64 rows, 33 MB 11.2 / 12.6, 68 MB 11.9 / 17.0; 8 over 8 of 64, 16 rows, 31 MB 9.5 / 11.3.
+    # In 32 bits the general kernel is the slower one from two rows behind 64 keys on (9 / 16, 16 rows of 2,000 27 / 232).
     LEAST_BYTES = 24e6
 
-    def __init__(self, group: int, page_size: int, key_bytes: int, tile_members: int):
-        """`key_bytes`: of one token's row(s) in one call's cache."""
+    def __init__(self, group: int, page_size: int, key_bytes: int, tile_members: int, least_bytes: float = 0):
+        """`key_bytes`: of one token's row(s) in one call's cache; `least_bytes`: what sets have to save, altogether."""
         self.group, self.page_size, self.key_bytes, self.tile_members = group, page_size, key_bytes, tile_members
+        self.least_bytes = least_bytes
         self.key = f"shared_beginnings_{group}"
         self._caches, self._plan, self._tiles = [], None, 0
 
@@ -185,7 +187,7 @@ class SharedBeginnings(BatchAnnotation):
             table[row, :n] = pages[:n]
         shared, members, tiles = sharing.plan(table, usable, self.page_size, self.tile_members)
         saved = int(shared.sum(dtype=np.int64)) - int(tiles[:, 2].sum(dtype=np.int64))
-        return (shared, members, tiles) if len(tiles) and saved * self.key_bytes >= self.LEAST_BYTES else None
+        return (shared, members, tiles) if len(tiles) and saved * self.key_bytes >= self.least_bytes else None
 
     def capacity(self, n_tokens, n_requests):
         return 6 * (-(-n_requests // 4) * 4)
