@@ -117,7 +117,7 @@ def run(b, scale, softcap=None, n_pad_tiles=0):
 # What an output element may be off.  32-bit: q.k has d products of 2^-24 each relative to sum |q k| <= |q| |k|; an error e of a
 # score changes a weight by e; |score * scale| errors stay below 2^-24 * (d / 2 + 4) * sum|qk| * scale, here sum|qk| * scale < 40
 # for all tests: 40 * 2^-24 * 132 < 3.2e-4 as a bound, and outputs are averages of |v| < 5.5: the bound is loose by the
-# square root of d (random signs), 2^-24 * 40 * 12 * 5.5 = 1.6e-4 stays one.  bfloat16: probabilities rounded to 2^-9 of themselves
+# square root of d (random signs), 2^-24 * 40 * 12 * 5.5 = 1.6e-4 stays one.  bfloat16: probabilities are rounded,
 # at most half a step 2^-8 relative, the sum of p |v| / sum p <= 5.5 at worst, on the average below 1; output rounded by 2^-8 |out|.
 def near(got, want, b):
     seen = [r for r in range(len(b["pos"])) if b["row_req"][r] >= 0]

@@ -14,7 +14,6 @@
 
 extern __shared__ __align__(1024) unsigned char fa_raw[];      // swizzle atoms: 1024-byte aligned
 
-
 __device__ __forceinline__ unsigned fa_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 // the word that a wait that ran out sets
 __device__ __forceinline__ unsigned fa_gave_up_at() { return fa_smem(fa_raw) + (unsigned)(kFaSmem - 4); }

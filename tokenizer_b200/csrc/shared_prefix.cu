@@ -10,7 +10,9 @@
 //
 // A block takes 32 (row, head) pairs, four a warp, and walks its piece 32 keys at a time: keys and values lie in shared
 // memory in 32 bits; a lane has a key for the scores (of its warp's four pairs at once, 16 multiply-adds for five 16-byte
-// reads of shared memory) and every 32nd lane of the head for the weighted values.
+// reads of shared memory) and every 32nd lane of the head for the weighted values.  8 rows of 14 heads of 64 lanes behind
+// 1,024 common keys, 32-bit: 16.8 us on the device, 2.5 a turn of 32 keys; 16 rows with 2,000 in common 27 us (232 where
+// every row reads all of its keys in the general attention).
 #include "common.cuh"
 
 #define SP_WARPS 8
