@@ -11,8 +11,8 @@ count of how much of that context the cache already holds.  One iteration:
     portions of their context, oldest first, under what is left of the token
     budget;
  3. reserve pages for those tokens, oldest request first.  When pages run out,
-    the newest running request loses all its pages and goes back to the front
-    of the waiting line; its context is run again later (nothing is sampled
+    the newest running request loses all its pages and goes back into the
+    waiting line, in front of younger ones; its context is run again later (nothing is sampled
     twice: a draw happens only when the whole context is in the cache).  A
     request that is alone and still does not fit fails;
  4. run the step, draw one id for each request whose context is now whole, let
@@ -138,9 +138,11 @@ class Scheduler:
 
     def _fork(self, r: _Request) -> List[_Request]:
         """The prompt of `r` is computed: fork the other answers to it, as many as there are batch slots and pages for (the
-        others join the line in front of younger requests).  Returns those that now run."""
+        others join the line in front of younger requests; all do where an older request waits).  Returns those that now run."""
         forks, r.forks = r.forks, []
         n = min(len(forks), self.max_batch_size - len(self.running), self.cache.can_fork(r.cache))
+        if self.waiting and self.waiting[0].id < forks[0].id:
+            n = 0
         for fork, cache in zip(forks, self.cache.fork(r.cache, [f.id for f in forks[:n]])):
             fork.cache = cache
             fork.published = True          # the prompt's pages are its parent's
@@ -151,6 +153,7 @@ class Scheduler:
         return forks[:n]
 
     def _wait_in_line(self, requests: List[_Request]) -> None:
+        """Requests of neighbouring ids join the line, which is in order of arrival, in front of younger ones."""
         younger = next((at for at, w in enumerate(self.waiting) if requests and w.id > requests[0].id), len(self.waiting))
         for at, r in enumerate(requests):
             self.waiting.insert(younger + at, r)
@@ -376,10 +379,8 @@ class Scheduler:
         victim.cache = None
         self.stats.preemptions += 1
         self.stats.last_preempted_id = victim.id
-        # To the front of the line.  Victims are taken newest first and every
-        # waiting request is newer than any running one, so the line stays in
-        # arrival order.
-        self.waiting.appendleft(victim)
+        # By its age: forks that wait for a slot can be older than a request that runs.
+        self._wait_in_line([victim])
 
     def _sample(self, ready: List[_Request], logits) -> None:
         now = time.perf_counter()
