@@ -3,8 +3,9 @@ import random
 
 import pytest
 
-from test_fork import ForkingEngine, alone, answers, finish
+from test_fork import CHUNK, FULL, STATE, WINDOW, ForkingEngine, alone, answers, finish, hold
 from tiny import random_ids
+from tokenizer_b200.cache import CachePlan, OutOfPages
 from tokenizer_b200.engine.generate import GenerateParams
 from tokenizer_b200.engine.scheduler import Scheduler
 
@@ -56,3 +57,38 @@ def test_a_preempted_request_does_not_pass_older_forks():
         s.add_request(random_ids(6, 50, 20 + at), GenerateParams(max_tokens=20))
     check_line(s)
     assert s.stats.preemptions > 0
+
+
+# ---- room for what follows a fork ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("needs", [[FULL], [FULL, WINDOW], [WINDOW, CHUNK, STATE]])
+@pytest.mark.parametrize("length", [3, 4, 8, 11, 24])
+@pytest.mark.parametrize("n_new", [0, 1, 5, 9])
+def test_as_many_forks_as_can_take_their_next_tokens(needs, length, n_new):
+    for pages in range(8, 24):
+        plan = CachePlan(needs, pages, 4, 12)
+        parent = hold(plan, "p", length)
+        n = plan.can_fork(parent, n_new)
+        children = plan.fork(parent, list(range(n)))
+        for child in children:
+            plan.reserve(child, n_new)
+        plan.check()
+        if n < 11:                               # pages are what is short: one more would not do
+            try:
+                more, = plan.fork(parent, ["more"])
+            except OutOfPages:
+                continue
+            assert not plan.can_reserve(more, n_new)
+
+
+def test_forks_leave_the_pages_that_others_need_next():
+    """A prompt that ends on a page's end, a younger request in the middle of its answer, few pages left."""
+    for pages in range(5, 14):
+        s = Scheduler(Engine(num_pages=pages), max_batch_size=8, token_budget=64)
+        ids = s.add_samples(random_ids(8, 50, 1), answers(6))
+        young = s.add_request(random_ids(3, 50, 2), GenerateParams(max_tokens=5))
+        s.step()
+        needed = sum(s.cache.pages_missing(r.cache, 1)[0] for r in s.running)
+        assert len(s.running) >= 2 and needed <= s.cache.allocators[0].available, pages
+        out = finish(s)
+        assert [out[i].tokens for i in ids] == [alone(random_ids(8, 50, 1), p) for p in answers(6)]
+        assert out[young].tokens == alone(random_ids(3, 50, 2), GenerateParams(max_tokens=5))

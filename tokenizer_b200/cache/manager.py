@@ -203,11 +203,25 @@ class CachePlan:
         return cache.length
 
     # ---- forks ----------------------------------------------------------------------
-    def can_fork(self, parent: RequestCache) -> int:
-        """How many forks of `parent` the request slots and the pages allow now."""
+    def pages_for_fork(self, parent: RequestCache, n_new: int = 1) -> List[int]:
+        """Per group, the pages that a fork of `parent` takes: the copy of the begun page, and those of its next `n_new`
+        tokens."""
+        full, begun = divmod(parent.length, self.page_size)
+        end_block = pages_for(parent.length + n_new, self.page_size)
+        needed = []
+        for g in range(len(self.groups)):
+            behind = range(full, full + 1 if begun else full)              # the begun page, where no token asks for it
+            wanted = set(self.wanted_blocks(g, parent.length, end_block)) | set(behind)
+            needed.append(sum(1 for b in wanted if b >= full or parent.tables[g][b] < 0))
+        return needed
+
+    def can_fork(self, parent: RequestCache, n_new: int = 1, beside: Sequence[int] = ()) -> int:
+        """How many forks of `parent` the request slots and the pages allow now, if each of them is to take `n_new` more
+        tokens and `beside` pages a group are left for others."""
         most = len(self._free_slots)
-        if parent.length % self.page_size:
-            most = min([most] + [a.available for a in self.allocators])
+        for g, (needed, allocator) in enumerate(zip(self.pages_for_fork(parent, n_new), self.allocators)):
+            if needed:
+                most = min(most, max(0, allocator.available - (beside[g] if beside else 0)) // needed)
         return most
 
     def fork(self, parent: RequestCache, request_ids: Sequence[object]) -> List[RequestCache]:
@@ -219,8 +233,8 @@ class CachePlan:
             raise ValueError("the request is closed")
         if len(set(ids)) < len(ids) or any(i in self.requests for i in ids):
             raise ValueError("a fork has a request id of its own")
-        if len(ids) > self.can_fork(parent):
-            raise OutOfPages(f"{len(ids)} forks of request {parent.request_id!r}: slots and pages are left for {self.can_fork(parent)}")
+        if len(ids) > self.can_fork(parent, 0):
+            raise OutOfPages(f"{len(ids)} forks of request {parent.request_id!r}: slots and pages are left for {self.can_fork(parent, 0)}")
         full, begun = divmod(parent.length, self.page_size)
         children = [self.open(i) for i in ids]
         copies: List[List[tuple]] = [[] for _ in self.groups]       # per group (page, its copy, rows)

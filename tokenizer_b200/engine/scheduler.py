@@ -140,7 +140,7 @@ class Scheduler:
         """The prompt of `r` is computed: fork the other answers to it, as many as there are batch slots and pages for (the
         others join the line in front of younger requests; all do where an older request waits).  Returns those that now run."""
         forks, r.forks = r.forks, []
-        n = min(len(forks), self.max_batch_size - len(self.running), self.cache.can_fork(r.cache))
+        n = min(len(forks), self.max_batch_size - len(self.running), self._room_for_forks(r.cache, 1))
         if self.waiting and self.waiting[0].id < forks[0].id:
             n = 0
         for fork, cache in zip(forks, self.cache.fork(r.cache, [f.id for f in forks[:n]])):
@@ -151,6 +151,12 @@ class Scheduler:
         self._wait_in_line(forks[n:])
         self.stats.forked += n
         return forks[:n]
+
+    def _room_for_forks(self, source: RequestCache, n_new: int) -> int:
+        """How many forks of `source` can each take `n_new` tokens beside what the running requests still need: the rest of
+        their contexts, or their next token."""
+        needed = [self.cache.pages_missing(r.cache, max(1, len(r.context) - r.cache.length)) for r in self.running]
+        return self.cache.can_fork(source, n_new, [sum(group) for group in zip(*needed)])
 
     def _wait_in_line(self, requests: List[_Request]) -> None:
         """Requests of neighbouring ids join the line, which is in order of arrival, in front of younger ones."""
