@@ -92,7 +92,8 @@ def generate_samples(model_or_engine, prompt: Sequence[int], n: int,
                      on_chunk: Optional[Callable[[int, str], Control]] = None,
                      max_batch_size: int = 64, token_budget: int = 2048, page_size: int = 16) -> List[Generated]:
     """`n` answers to one prompt.  The prompt is computed once; the others are forked from its cache (its full pages shared,
-    the begun one copied) and decode beside it, the common keys read once a step for all of them where that pays.  One
+    the begun one copied) and decode beside it, the common keys read once a step for all of them where that pays.  Answers
+    beyond `max_batch_size` are forked when others have ended.  One
     GenerateParams stands for all (answer i draws with its seed + i), or one each; `on_chunk(index, text)` may return
     Control.STOP."""
     if n < 1:
@@ -103,9 +104,10 @@ def generate_samples(model_or_engine, prompt: Sequence[int], n: int,
     else:
         batch = max(1, min(max_batch_size, n))
         own = max((q.max_tokens for q in each), default=0) // page_size + 2       # pages behind the prompt's full ones
-        engine = engine_for(model_or_engine, (len(prompt) // page_size + batch * own) * page_size, page_size, max_requests=batch,
-                            shared_attention=True)
-    scheduler = Scheduler(engine, max_batch_size=min(max_batch_size, engine.cache.max_requests), token_budget=token_budget)
+        kept = 1 if n > batch else 0           # a slot and a begun page for the prompt that waiting answers are forked from
+        engine = engine_for(model_or_engine, (len(prompt) // page_size + batch * own + kept) * page_size, page_size,
+                            max_requests=batch + kept, shared_attention=True)
+    scheduler = Scheduler(engine, max_batch_size=min(max_batch_size, n, engine.cache.max_requests), token_budget=token_budget)
     ids = scheduler.add_samples(prompt, each, token_bytes, on_chunk)
     results = scheduler.run()
     return [results[i] for i in ids]

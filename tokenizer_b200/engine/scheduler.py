@@ -33,8 +33,11 @@ host's share of a step is paid once a burst.  When the pool has no pages for the
 whole burst the iteration runs a single step as above.
 
 Several answers to one prompt (`add_samples`) are requests of their own of which the first runs the prompt.  When its last
-token has been computed the others are forked from its cache and draw their first ids from the same logits; those that no
-batch slot or page is left for wait in line as any request does, and find the prompt's full pages shared.
+token has been computed all of them draw their first ids from the same logits, and the others are forked from its cache.
+Those that no batch slot or page is left for wait in line.  Where the cache shares prefixes they find the prompt's full
+pages when their turn comes and compute its begun page again.  Where it does not (windows, chunks, states), the last of them
+waits with a fork of its own, in a request slot beside the batch, from which the others are forked when their turn comes:
+the prompt is not computed again unless nothing else can go on without the pages that are kept so, or no slot is to be had.
 
 The reference's scheduler (qwen-server/src/engine.rs:229-402, 455-704) admits
 and preempts in the same way but runs a whole prompt per iteration; the token
@@ -47,7 +50,7 @@ from collections import deque
 from dataclasses import dataclass, field
 from typing import Callable, Deque, Dict, List, Optional, Sequence
 
-from ..cache.manager import OutOfPages
+from ..cache.manager import OutOfPages, RequestCache
 from .batch import StepEntry
 from .generate import Control, Generated, GenerateParams, SampleCursor, StopReason
 
@@ -78,6 +81,8 @@ class _Request:
     arrived: float = 0.0
     prompt_done: Optional[float] = None
     forks: List["_Request"] = field(default_factory=list)    # the other answers to its prompt, until it is computed
+    keeps_prompt: bool = False    # it waits, and its cache holds the prompt for those that wait beside it
+    keeper: Optional["_Request"] = None                      # the one of them that does
 
 
 class Scheduler:
@@ -136,27 +141,54 @@ class Scheduler:
         self.waiting.append(made[0])
         return [r.id for r in made]
 
-    def _fork(self, r: _Request) -> List[_Request]:
-        """The prompt of `r` is computed: fork the other answers to it, as many as there are batch slots and pages for (the
-        others join the line in front of younger requests; all do where an older request waits).  Returns those that now run."""
+    def _fork(self, r: _Request, logits, row: int) -> List[_Request]:
+        """The prompt of `r` is computed, its logits are `logits[row]`: fork the other answers to it, as many as there are
+        batch slots and pages for (none where an older request waits).  The others draw their first ids and join the line
+        in front of younger requests; the last of them keeps the prompt if nothing else does.  Returns those that now run."""
         forks, r.forks = r.forks, []
-        n = min(len(forks), self.max_batch_size - len(self.running), self._room_for_forks(r.cache, 1))
+        room = self._room_for_forks(r.cache, 1)
+        n = min(len(forks), self.max_batch_size - len(self.running), room)
         if self.waiting and self.waiting[0].id < forks[0].id:
             n = 0
-        for fork, cache in zip(forks, self.cache.fork(r.cache, [f.id for f in forks[:n]])):
+        for fork in forks:
+            fork.prompt_done = r.prompt_done
+        later = self._first_ids(forks[n:], logits, row)
+        if later and not self.cache.share_prefixes:
+            if room == n and n > 1:
+                n -= 1                     # a place in the batch for the prompt
+                later = self._first_ids([forks[n]], logits, row) + later
+            later[-1].keeps_prompt = room > n
+        holders = forks[:n] + [f for f in later if f.keeps_prompt]
+        for fork, cache in zip(holders, self.cache.fork(r.cache, [f.id for f in holders])):
             fork.cache = cache
             fork.published = True          # the prompt's pages are its parent's
-            fork.prompt_done = r.prompt_done
-            self.running.append(fork)
-        self._wait_in_line(forks[n:])
-        self.stats.forked += n
+        for fork in later[:-1]:
+            fork.keeper = later[-1]
+        self.running += forks[:n]
+        self._wait_in_line(later)
+        self.stats.forked += len(holders)
         return forks[:n]
+
+    def _first_ids(self, forks: List[_Request], logits, row: int) -> List[_Request]:
+        """Answers that wait draw their first ids, a batch at a time.  Returns those that did not end with them."""
+        for at in range(0, len(forks), self.max_batch_size):
+            drawing = [f for f in forks[at:at + self.max_batch_size] if f.cursor.wants_sample()]
+            if drawing:
+                self._accept(drawing, self.engine.sample(*self._draw(logits[[row] * len(drawing)], drawing)))
+        for f in forks:
+            if f.cursor.done is not None:
+                self._retire(f, f.prompt_done)
+        return [f for f in forks if f.cursor.done is None]
 
     def _room_for_forks(self, source: RequestCache, n_new: int) -> int:
         """How many forks of `source` can each take `n_new` tokens beside what the running requests still need: the rest of
         their contexts, or their next token."""
+        return self.cache.can_fork(source, n_new, self._pages_needed())
+
+    def _pages_needed(self) -> List[int]:
+        """Per group, the pages that the running requests lack for the rest of their contexts or their next token."""
         needed = [self.cache.pages_missing(r.cache, max(1, len(r.context) - r.cache.length)) for r in self.running]
-        return self.cache.can_fork(source, n_new, [sum(group) for group in zip(*needed)])
+        return [sum(group) for group in zip(*needed)] or [0] * len(self.cache.allocators)
 
     def _wait_in_line(self, requests: List[_Request]) -> None:
         """Requests of neighbouring ids join the line, which is in order of arrival, in front of younger ones."""
@@ -316,17 +348,51 @@ class Scheduler:
                 self._fail(head, f"the cache has {self.cache.num_pages} pages of "
                                  f"{self.cache.page_size}; this request needs {self._context_pages(head)}")
                 continue
-            try:
-                cache = self.cache.open(head.id)
-            except OutOfPages:
-                break                    # every request slot is held (some outside this scheduler): wait
-            adopted = self.cache.adopt_prefix(cache, head.context[:-1])
-            if not self.cache.can_reserve(cache, len(head.context) - cache.length):
-                self.cache.close(cache)
-                break
-            self.stats.shared_prefix_tokens += adopted
-            head.cache = cache
-            self.running.append(self.waiting.popleft())
+            if self._open(head):
+                self.running.append(self.waiting.popleft())
+            elif self.running or not self._give_up_prompt():
+                break                    # no pages, or every request slot is held (some outside this scheduler): wait
+
+    def _open(self, r: _Request) -> bool:
+        """A cache for the head of the line: the prompt that it keeps, a fork of one that is kept for it, or a fresh one on
+        what is found of its beginning.  False: there is no slot, or there are not the pages for its context."""
+        if r.keeps_prompt:
+            missing = self.cache.pages_missing(r.cache, len(r.context) - r.cache.length)
+            if any(m + n > a.available for m, n, a in zip(missing, self._pages_needed(), self.cache.allocators)):
+                return False
+            r.keeps_prompt = False
+            return True
+        if r.keeper is not None and r.keeper.keeps_prompt:
+            prompt = r.keeper.cache
+            if self._room_for_forks(prompt, len(r.context) - prompt.length) < 1:
+                return False
+            r.cache, = self.cache.fork(prompt, [r.id])
+            r.published = True
+            self.stats.forked += 1
+            return True
+        try:
+            cache = self.cache.open(r.id)
+        except OutOfPages:
+            return False
+        adopted = self.cache.adopt_prefix(cache, r.context[:-1])
+        if not self.cache.can_reserve(cache, len(r.context) - cache.length):
+            self.cache.close(cache)
+            return False
+        self.stats.shared_prefix_tokens += adopted
+        r.cache = cache
+        return True
+
+    def _give_up_prompt(self) -> bool:
+        """Nothing can go on: give back the prompt that was kept last.  False: none is kept."""
+        for r in reversed(self.waiting):
+            if r.keeps_prompt:
+                self._drop_prompt(r)
+                return True
+        return False
+
+    def _drop_prompt(self, r: _Request) -> None:
+        self.cache.close(r.cache)
+        r.cache, r.keeps_prompt = None, False
 
     def _adopt_late(self, r: _Request) -> None:
         """A running request that holds nothing yet looks once more for pages that hold the
@@ -372,6 +438,8 @@ class Scheduler:
                 return shares
             victim = max(self.running, key=lambda r: r.id)
             if victim is short and len(self.running) == 1:
+                if self._give_up_prompt():
+                    continue
                 self.running.remove(short)
                 self.cache.close(short.cache)
                 self._fail(short, f"the cache has {self.cache.num_pages} pages of "
@@ -398,7 +466,7 @@ class Scheduler:
             if not r.published and r.cache.length >= len(r.prompt):
                 self.cache.publish_prompt(r.cache, r.prompt)
                 r.published = True
-            same_row = [r] + (self._fork(r) if r.forks else [])
+            same_row = [r] + (self._fork(r, logits, row) if r.forks else [])
             forked += same_row[1:]
             for request in same_row:
                 if request.cursor.wants_sample():
@@ -407,11 +475,7 @@ class Scheduler:
         ready = ready + forked
         if drawing:
             picked = logits if rows == list(range(computed)) else logits[rows]
-            draw = [picked, [r.cursor.params.temperature for r in drawing],
-                    [r.cursor.params.top_p for r in drawing],
-                    [r.cursor.next_uniform() for r in drawing]]
-            if any(r.cursor.params.top_k > 0 or r.cursor.params.min_p > 0 for r in drawing):
-                draw += [[r.cursor.params.top_k for r in drawing], [r.cursor.params.min_p for r in drawing]]
+            draw = self._draw(picked, drawing)
             launch = getattr(self.engine, "sample_launch", None)
             if launch is None:
                 ids = self.engine.sample(*draw)
@@ -421,18 +485,31 @@ class Scheduler:
                     self._pack_ahead(ready)          # beside the device
                     self._launch_ahead(drawing, pending)
                 ids = pending.result()
-            self.stats.tokens_sampled += len(ids)
-            for r, token in zip(drawing, ids):
-                if r.cursor.accept(int(token)):
-                    r.context.append(int(token))
+            self._accept(drawing, ids)
         for r in ready:
             if r.cursor.done is not None:
                 self._retire(r, now)
 
+    @staticmethod
+    def _draw(logits, drawing: List[_Request]) -> List:
+        """What the engine's draw takes: a row of logits a request, and the requests' settings and numbers."""
+        params = [r.cursor.params for r in drawing]
+        draw = [logits, [p.temperature for p in params], [p.top_p for p in params], [r.cursor.next_uniform() for r in drawing]]
+        if any(p.top_k > 0 or p.min_p > 0 for p in params):
+            draw += [[p.top_k for p in params], [p.min_p for p in params]]
+        return draw
+
+    def _accept(self, drawing: List[_Request], ids) -> None:
+        self.stats.tokens_sampled += len(ids)
+        for r, token in zip(drawing, ids):
+            if r.cursor.accept(int(token)):
+                r.context.append(int(token))
+
     def _retire(self, r: _Request, now: float) -> None:
-        self.running.remove(r)
-        self.cache.close(r.cache)
-        r.cache = None
+        if r.cache is not None:            # not an answer that ended while it waited
+            self.running.remove(r)
+            self.cache.close(r.cache)
+            r.cache = None
         result = r.cursor.done
         result.prefill = (r.prompt_done or now) - r.arrived
         result.decode = time.perf_counter() - (r.prompt_done or now)
@@ -442,6 +519,8 @@ class Scheduler:
     def _fail(self, r: _Request, message: str) -> None:
         forks, r.forks = r.forks, []
         self._wait_in_line(forks)              # what it was refused for may not hold for them
+        if r.keeps_prompt:
+            self._drop_prompt(r)
         self.finished[r.id] = Generated(list(r.cursor.tokens), r.cursor.text, list(r.cursor.chunks),
                                         StopReason.FAILED, r.cursor.produced, error=message)
         self.stats.requests_failed += 1
