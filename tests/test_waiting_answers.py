@@ -224,3 +224,31 @@ def test_waiting_answers_of_every_kind_of_cache(module, name, tmp_path_factory):
     assert s.stats.tokens_run == len(prompt) + sum(len(a.tokens) - 1 for a in want)
     engine.cache.check()
     assert not engine.cache.requests
+
+
+@pytest.mark.parametrize("needs, share", [([FULL], True), ([FULL, STATE], False), ([FULL, WINDOW], False)])
+@pytest.mark.parametrize("lengths, samples, batch", [([41], 64, 8), ([40, 17, 3], 5, 4), ([9] * 6, 3, 2), ([5], 2, 8)])
+def test_the_command_line_sizes_its_pool_for_what_runs_together(needs, share, lengths, samples, batch, monkeypatch, tmp_path, capsys):
+    import tokenizer_b200 as tb
+    from tokenizer_b200 import cli
+    made = []
+
+    def engine(model, num_pages, page_size, max_requests, share_prefixes, shared_attention):
+        made.append(Engine(num_pages=num_pages, page_size=page_size, max_requests=max_requests, needs=needs, share_prefixes=share_prefixes))
+        return made[-1]
+
+    monkeypatch.setattr(tb, "Engine", engine)
+    monkeypatch.setattr(tb, "load_model", lambda *a, **kw: object())
+    monkeypatch.setattr(tb, "load_eos_token_ids", lambda folder: [])
+    prompts = [random_ids(n, 50, i) for i, n in enumerate(lengths)]
+    args = [a for p in prompts for a in ("--ids", ",".join(map(str, p)))]
+    assert cli.main(["--model", str(tmp_path), "--max-tokens", "9", "--temperature", "0.9", "--samples", str(samples), "--page-size", "4",
+                     "--max-batch-size", str(batch)] + args) == 0
+    lines = capsys.readouterr().out.strip().splitlines()
+    want = [alone(p, GenerateParams(max_tokens=9, temperature=0.9, seed=i)) for p in prompts for i in range(samples)]
+    assert lines == [" ".join(map(str, w)) for w in want]
+    # a prompt's full pages once, and tails of at most 3 + 9 tokens (a page more for the next one) for those that run or are kept
+    together = min(batch, len(prompts) * samples)
+    assert made[0].cache.num_pages <= sum(n // 4 for n in lengths) + together * 4 + len(prompts)
+    if not share:
+        assert tokens_run(made[0]) == sum(lengths) + len(want) * 8

@@ -86,6 +86,16 @@ def sample_params(params: Union[GenerateParams, Sequence[GenerateParams]], n: in
     return list(params)
 
 
+def samples_room(lengths: Sequence[int], max_tokens: int, samples: int, batch: int, page_size: int):
+    """(pages, request slots) for `samples` answers to each of the prompts of these lengths, at most `batch` of them at once:
+    the prompts' full pages once, what lies behind those for a batch, and where answers wait a begun page and a slot for
+    every prompt that may be kept for them."""
+    together = max(1, min(batch, len(lengths) * samples))
+    kept = min(batch, len(lengths)) if samples > 1 and len(lengths) * samples > batch else 0
+    behind = max_tokens // page_size + 2                # pages behind a prompt's full ones
+    return sum(n // page_size for n in lengths) + together * behind + kept, together + kept
+
+
 def generate_samples(model_or_engine, prompt: Sequence[int], n: int,
                      params: Union[GenerateParams, Sequence[GenerateParams]],
                      token_bytes: Optional[Callable[[int], bytes]] = None,
@@ -102,11 +112,8 @@ def generate_samples(model_or_engine, prompt: Sequence[int], n: int,
     if hasattr(model_or_engine, "step") and hasattr(model_or_engine, "cache"):
         engine = model_or_engine
     else:
-        batch = max(1, min(max_batch_size, n))
-        own = max((q.max_tokens for q in each), default=0) // page_size + 2       # pages behind the prompt's full ones
-        kept = 1 if n > batch else 0           # a slot and a begun page for the prompt that waiting answers are forked from
-        engine = engine_for(model_or_engine, (len(prompt) // page_size + batch * own + kept) * page_size, page_size,
-                            max_requests=batch + kept, shared_attention=True)
+        pages, requests = samples_room([len(prompt)], max((q.max_tokens for q in each), default=0), n, max_batch_size, page_size)
+        engine = engine_for(model_or_engine, pages * page_size, page_size, max_requests=requests, shared_attention=True)
     scheduler = Scheduler(engine, max_batch_size=min(max_batch_size, n, engine.cache.max_requests), token_budget=token_budget)
     ids = scheduler.add_samples(prompt, each, token_bytes, on_chunk)
     results = scheduler.run()

@@ -6,7 +6,8 @@ tokenizer.json, or ids with --ids.
 
 Beyond the reference's options: several prompts (positional arguments or `--ids` given more
 than once) run together through the scheduler, and the scheduler's and the cache's sizes can
-be set: --num-pages N (pages of the cache; default: room for every prompt to its end),
+be set: --num-pages N (pages of the cache; default: room for every prompt to its end, with --samples for
+every prompt and for the answers that run together),
 --page-size N (tokens a page, default 16), --max-batch-size N (requests that run together,
 default 8 as the reference's server: qwen-server/src/lib.rs:47-55), --token-budget N (tokens a
 step may run: prompts are cut into portions under it; default 2048).  --num-blocks,
@@ -168,11 +169,13 @@ def main(argv=None) -> int:
         params.validate()
         model = tb.load_model(folder, dtype=args["dtype"], device=args["device"])
         page = args["page_size"]
-        pages = args["num_pages"]
-        if pages is None:
-            pages = samples * sum(-(-(len(ids) + params.max_tokens + 1) // page) for ids in prompts)
         batch = min(args["max_batch_size"], len(prompts) * samples)
-        engine = tb.Engine(model, num_pages=pages, page_size=page, max_requests=batch,
+        pages, requests = sum(-(-(len(ids) + params.max_tokens + 1) // page) for ids in prompts), batch
+        if samples > 1:
+            pages, requests = tb.api.samples_room([len(ids) for ids in prompts], params.max_tokens, samples, batch, page)
+        if args["num_pages"] is not None:
+            pages = args["num_pages"]
+        engine = tb.Engine(model, num_pages=pages, page_size=page, max_requests=requests,
                            share_prefixes=True, shared_attention=samples > 1)
         started = time.perf_counter()
         token_bytes = (lambda t: tokenizer.decode_bytes([t])) if tokenizer else None
