@@ -198,7 +198,7 @@ def raise_if_error(where: str = "") -> None:
         return
     _error_word[0].value = 0
     library, reason = _LIBRARY_NAMES.get(code // 16, f"library {code // 16}"), code % 16
-    if reason == 2 and code // 16 == 2:
+    if reason == 2 and code // 16 in (2, 7):             # their blocks do not wait on one another
         text = "a shared-memory base was not aligned as the kernel needs"
     else:
         text = _REASONS.get(reason, f"reason {reason}")
