@@ -2,6 +2,7 @@
 import ctypes
 
 import pytest
+import torch
 
 from tokenizer_b200.kernels import ops
 
@@ -14,3 +15,37 @@ def test_an_unaligned_base_is_called_that(monkeypatch):
     with pytest.raises(ops.KernelError, match="shared_prefix_tcgen05: .*not aligned"):
         ops.raise_if_error()
     assert value.value == 0
+
+
+def call(b, members=None, tiles=None):
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    out = torch.zeros_like(b["q"]).cuda()
+    ops.shared_prefix_attention(b["q"].cuda(), b["k"].cuda(), b["v"].cuda(), out, b["table"].cuda(), ints(b["row_req"]), ints(b["pos"]),
+                                ints(b["shared"]), ints(b["members"] if members is None else members),
+                                ints(b["tiles"] if tiles is None else tiles).view(-1, 4), b["nh"], b["nkv"], b["d"], b["page"], 0.125)
+    torch.cuda.synchronize()
+    return out.view(-1, b["nh"], b["d"]).double().cpu()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("nh, nkv, d", [(14, 2, 64), (12, 2, 128), (6, 1, 20)])
+def test_tiles_that_are_none_raise(nh, nkv, d, dtype, monkeypatch):
+    """Too many members, members behind the list's end or in front of its beginning, rows that the batch does not have."""
+    from test_shared_prefix import make, near, plain
+    monkeypatch.setattr(ops, "SHARED_PREFIX_LITTLE", 0)
+    most = ops.shared_prefix_tile_members(nh, nkv)
+    b = make(nh, nkv, d, 16, [(most + 1, 3)], 1, [9, 20], dtype)
+    rows, keys, want = b["members"], 48, plain(b, 0.125)
+    assert len(b["tiles"]) == 2
+    ops.raise_if_error()
+    near(call(b), want, b)
+    ops.raise_if_error()
+    for members, tiles in [(rows, [[0, most + 1, keys, 0]]), (rows, [[0, most, keys, 0], [most, 2, keys, 0]]),
+                           (rows, [[-1, 2, keys, 0]]), (rows, [[2 ** 31 - 1, 2, keys, 0]]), ([], [[0, 1, keys, 0]]),
+                           (rows[:-1] + [most + 2], b["tiles"]), ([2 ** 31 - 1] + rows[1:], b["tiles"])]:
+        call(b, members, tiles)
+        with pytest.raises(ops.KernelError, match="shared_prefix.*tile"):
+            ops.raise_if_error()
+    near(call(b), want, b)
+    ops.raise_if_error()

@@ -44,6 +44,7 @@ enum : int {
   TOKB200_LIB_LAYER_SMALL_M = 5,
   TOKB200_LIB_GEMM_F32_TCGEN05 = 6,
   TOKB200_LIB_SHARED_PREFIX_TCGEN05 = 7,
+  TOKB200_LIB_SHARED_PREFIX = 8,
 };
 __device__ int* tokb200_error_word = nullptr;
 

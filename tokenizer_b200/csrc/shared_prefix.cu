@@ -36,12 +36,18 @@ __device__ __forceinline__ float sp_warp_max(float v) {      // one instruction;
   return m;
 }
 
+// whether a tile has at most `most` members, all of them in a list of `n_listed`
+__device__ __forceinline__ bool sp_tile_fits(const int4& tile, int most, int n_listed) {
+  return tile.y <= 0 || (tile.y <= most && tile.x >= 0 && tile.x <= n_listed - tile.y);
+}
+
 // the request whose table a tile's keys are read through: its first live member's (-1: it has none)
-__device__ __forceinline__ int sp_tile_request(const int4& tile, const int* __restrict__ members, const int* __restrict__ row_req) {
+__device__ __forceinline__ int sp_tile_request(const int4& tile, const int* __restrict__ members, const int* __restrict__ row_req, int n_rows) {
   int req = -1;
   for (int i = 0; i < tile.y && req < 0; ++i) {
     const int row = members[tile.x + i];
-    req = row < 0 ? -1 : row_req[row];
+    if (row >= n_rows && threadIdx.x == 0) tokb200_report_error(TOKB200_LIB_SHARED_PREFIX, 3);
+    req = row < 0 || row >= n_rows ? -1 : row_req[row];
   }
   return req;
 }
@@ -52,8 +58,9 @@ __global__ void __launch_bounds__(SP_THREADS, DI <= 4 ? 2 : 1)
 shared_prefix_parts_kernel(const T* __restrict__ q, const T* __restrict__ k_pool, const T* __restrict__ v_pool,
                            const int* __restrict__ block_table, int table_stride, const int* __restrict__ row_req,
                            const int* __restrict__ pos, const int* __restrict__ shared, const int* __restrict__ members,
-                           const int4* __restrict__ tiles, int n_tiles, int nh, int nkv, int d, int page, float scale_log2,
-                           float cap_in, float cap_out, int tile_chunks, int row_chunks, int tile_pieces, int own_pieces, float* __restrict__ parts) {
+                           const int4* __restrict__ tiles, int n_tiles, int tile_members, int n_listed, int n_rows, int nh, int nkv,
+                           int d, int page, float scale_log2, float cap_in, float cap_out, int tile_chunks,
+                           int row_chunks, int tile_pieces, int own_pieces, float* __restrict__ parts) {
   constexpr int kD = DI * 32, kStride = kD + 4;
   extern __shared__ __align__(16) float sp_smem[];
   float* q_s = sp_smem;                              // [pair][kD]
@@ -73,9 +80,13 @@ shared_prefix_parts_kernel(const T* __restrict__ q, const T* __restrict__ k_pool
   const int row_alone = common ? -1 : unit;
   if (common) {
     const int4 tile = tiles[unit];
+    if (!sp_tile_fits(tile, tile_members, n_listed)) {
+      if (threadIdx.x == 0) tokb200_report_error(TOKB200_LIB_SHARED_PREFIX, 3);
+      return;
+    }
     first_member = tile.x;
     n_pairs = tile.y * group;
-    req = sp_tile_request(tile, members, row_req);
+    req = sp_tile_request(tile, members, row_req, n_rows);
     const int keys = min(tile.z, table_stride * page), len = sp_piece(keys, tile_pieces);
     first = piece * len;
     end = min(keys, first + len);
@@ -95,6 +106,10 @@ shared_prefix_parts_kernel(const T* __restrict__ q, const T* __restrict__ k_pool
   for (int i = 0; i < SP_PAIRS_WARP; ++i) {
     const int pair = chunk * SP_PAIRS + warp * SP_PAIRS_WARP + i;
     row[i] = pair < n_pairs ? row_of(pair) : -1;
+    if (row[i] >= n_rows) {
+      tokb200_report_error(TOKB200_LIB_SHARED_PREFIX, 3);
+      row[i] = -1;
+    }
     head[i] = kvh * group + pair % group;
   }
   {
@@ -257,7 +272,7 @@ TOKB200_API int tokb200_shared_prefix_pieces(int n_rows, int n_tiles, int nkv, i
 
 template <typename T, int DI>
 static int sp_launch(const void* q, const void* k_pool, const void* v_pool, void* out, const int* block_table, int table_stride,
-                     const int* row_req, const int* pos, const int* shared, const int* members, const int* tiles, int n_tiles,
+                     const int* row_req, const int* pos, const int* shared, const int* members, int n_listed, const int* tiles, int n_tiles,
                      int tile_members, int n_rows, int nh, int nkv, int d, int page, float scale, const float* sink, float softcap,
                      int tile_pieces, int own_pieces, float* parts, cudaStream_t stream) {
   const int group = nh / nkv;
@@ -276,8 +291,8 @@ static int sp_launch(const void* q, const void* k_pool, const void* v_pool, void
   }
   const dim3 grid(tile_pieces > own_pieces ? tile_pieces : own_pieces, nkv, (unsigned)units);
   int status = launch_dependent(shared_prefix_parts_kernel<T, DI>, grid, dim3(SP_THREADS), smem, stream, (const T*)q, (const T*)k_pool,
-                                (const T*)v_pool, block_table, table_stride, row_req, pos, shared, members, (const int4*)tiles, n_tiles, nh,
-                                nkv, d, page, scale * SP_LOG2E, softcap > 0.f ? scale / softcap : 0.f,
+                                (const T*)v_pool, block_table, table_stride, row_req, pos, shared, members, (const int4*)tiles, n_tiles,
+                                tile_members, n_listed, n_rows, nh, nkv, d, page, scale * SP_LOG2E, softcap > 0.f ? scale / softcap : 0.f,
                                 softcap > 0.f ? softcap * SP_LOG2E : 0.f, tile_chunks, row_chunks, tile_pieces, own_pieces, parts);
   if (status != TOKB200_OK) return status;
   constexpr int kPairs = SP_JOIN_THREADS / 32;
@@ -285,20 +300,21 @@ static int sp_launch(const void* q, const void* k_pool, const void* v_pool, void
                           stream, parts, row_req, pos, shared, n_rows, nh, d, table_stride * page, tile_pieces, own_pieces, sink, (T*)out);
 }
 
-// tiles: [n_tiles][4] = (first place in `members`, members, keys, 0); at most `tile_members` members each.
+// tiles: [n_tiles][4] = (first place in `members`, members, keys, 0); at most `tile_members` members each, out of `n_listed`.  A tile
+// that is not so, or a member that is not a row, computes nothing and sets the error word.
 TOKB200_API int tokb200_shared_prefix_attention(
     const void* q, const void* k_pool, const void* v_pool, void* out, int dtype, const int* block_table, int table_stride,
-    const int* row_req, const int* pos, const int* shared, const int* members, const int* tiles, int n_tiles, int tile_members,
-    int n_rows, int nh, int nkv, int d, int page, float scale, const float* sink, float softcap, int tile_pieces, int own_pieces,
+    const int* row_req, const int* pos, const int* shared, const int* members, int n_listed, const int* tiles, int n_tiles,
+    int tile_members, int n_rows, int nh, int nkv, int d, int page, float scale, const float* sink, float softcap, int tile_pieces, int own_pieces,
     float* parts, cudaStream_t stream) {
   if (n_rows <= 0) return TOKB200_OK;
-  if (nh <= 0 || nkv <= 0 || nh % nkv || d <= 0 || d > 256 || page <= 0 || n_tiles < 0 || tile_members < 1 || tile_pieces < 1 || own_pieces < 1 ||
+  if (nh <= 0 || nkv <= 0 || nh % nkv || d <= 0 || d > 256 || page <= 0 || n_tiles < 0 || n_listed < 0 || tile_members < 1 || tile_pieces < 1 || own_pieces < 1 ||
       tile_pieces > 65535 || table_stride <= 0 || (long long)table_stride * page > 0x7fffffffLL || (long long)n_rows * nh > 0x7fffffffLL)
     return TOKB200_BAD_SIZE;
   if ((uintptr_t)tiles & 15) return TOKB200_BAD_ALIGNMENT;
 #define SP_CASE(T, DI)                                                                                                             \
-  return sp_launch<T, DI>(q, k_pool, v_pool, out, block_table, table_stride, row_req, pos, shared, members, tiles, n_tiles, tile_members, \
-                          n_rows, nh, nkv, d, page, scale, sink, softcap, tile_pieces, own_pieces, parts, stream)
+  return sp_launch<T, DI>(q, k_pool, v_pool, out, block_table, table_stride, row_req, pos, shared, members, n_listed, tiles, n_tiles, \
+                          tile_members, n_rows, nh, nkv, d, page, scale, sink, softcap, tile_pieces, own_pieces, parts, stream)
 #define SP_TYPE(T)                                                                                                                 \
   do {                                                                                                                             \
     if (d <= 32) SP_CASE(T, 1);                                                                                                    \

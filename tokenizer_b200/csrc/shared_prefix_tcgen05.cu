@@ -58,12 +58,18 @@ __host__ __device__ __forceinline__ int sp_piece(int n, int pieces) {
   return len < SP_KEYS ? SP_KEYS : len;
 }
 
+// whether a tile has at most `most` members, all of them in a list of `n_listed`
+__device__ __forceinline__ bool sp_tile_fits(const int4& tile, int most, int n_listed) {
+  return tile.y <= 0 || (tile.y <= most && tile.x >= 0 && tile.x <= n_listed - tile.y);
+}
+
 // the request whose table a tile's keys are read through: its first live member's (-1: it has none)
-__device__ __forceinline__ int sp_tile_request(const int4& tile, const int* __restrict__ members, const int* __restrict__ row_req) {
+__device__ __forceinline__ int sp_tile_request(const int4& tile, const int* __restrict__ members, const int* __restrict__ row_req, int n_rows) {
   int req = -1;
   for (int i = 0; i < tile.y && req < 0; ++i) {
     const int row = members[tile.x + i];
-    req = row < 0 ? -1 : row_req[row];
+    if (row >= n_rows && threadIdx.x == 0) tokb200_report_error(TOKB200_LIB_SHARED_PREFIX_TCGEN05, 3);
+    req = row < 0 || row >= n_rows ? -1 : row_req[row];
   }
   return req;
 }
@@ -74,8 +80,8 @@ __global__ void __launch_bounds__(SP_THREADS, 1)
 shared_prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                              const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ v_pool,
                              const int* __restrict__ block_table, int table_stride, const int* __restrict__ row_req,
-                             const int* __restrict__ members, const int4* __restrict__ tiles, int nh, int nkv, int page, int run,
-                             int pool_rows, int pieces, float scale_log2, float cap_in, float cap_out,
+                             const int* __restrict__ members, int n_listed, const int4* __restrict__ tiles, int n_rows, int nh, int nkv, int page,
+                             int run, int pool_rows, int pieces, float scale_log2, float cap_in, float cap_out,
                              float* __restrict__ acc_parts, float2* __restrict__ stat_parts) {
   unsigned char* q_s = fa_raw;                                   // lane 0, lane 1
   unsigned char* ring = q_s + 2 * kTileBytes;
@@ -116,7 +122,10 @@ shared_prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __
   pdl_wait();
   pdl_launch();
   const int4 tile = tiles[blockIdx.z];
-  const int req = sp_tile_request(tile, members, row_req);
+  const int lane_members = SP_ROWS / group;            // members a lane
+  const bool fits = sp_tile_fits(tile, 2 * lane_members, n_listed);
+  if (!fits && threadIdx.x == 0) tokb200_report_error(TOKB200_LIB_SHARED_PREFIX_TCGEN05, 3);
+  const int req = fits ? sp_tile_request(tile, members, row_req, n_rows) : -1;
   const bool aligned = (fa_smem(fa_raw) & 1023u) == 0;
   if (!aligned && threadIdx.x == 0) {
     atomicExch(&sp_error_flag, 2);
@@ -126,9 +135,8 @@ shared_prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __
   const int first = piece * len, end = min(keys, first + len);
   const bool live = aligned && req >= 0 && first < end;
   const int n_blocks = live ? (end - first + SP_KEYS - 1) / SP_KEYS : 0;
-  // members a lane; a tile that one lane holds is split along its keys
-  const int lane_members = SP_ROWS / group, n_members = min(tile.y, 2 * lane_members);
-  const bool split = n_members <= lane_members;
+  const int n_members = tile.y;
+  const bool split = n_members <= lane_members;      // a tile that one lane holds is split along its keys
   auto rows_of = [&](int l) { return group * (split || l == 0 ? min(n_members, lane_members) : n_members - lane_members); };
   auto member_of = [&](int l, int r) { return members[tile.x + (split ? 0 : l * lane_members) + r / group]; };
   auto steps_of = [&](int l) { return split ? (n_blocks + 1 - l) / 2 : n_blocks; };
@@ -276,7 +284,11 @@ shared_prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __
     float* my_stat = stat_s + (l * 2 + half) * SP_ROWS + r;
     const float* other_stat = stat_s + (l * 2 + 1 - half) * SP_ROWS + r;
     auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + l * 4 + (warp & 3)) : "memory"); };
-    const int row = r < rows_of(l) ? member_of(l, r) : -1;
+    int row = r < rows_of(l) ? member_of(l, r) : -1;
+    if (row >= n_rows) {
+      tokb200_report_error(TOKB200_LIB_SHARED_PREFIX_TCGEN05, 3);
+      row = -1;
+    }
     if (!split || l == 0) {
       // the rows of q that the warp's lanes own, half of a row's lanes a warp, 16 bytes a load; behind the members: zeros
       constexpr int kPieces = HEAD_DIM / 16, kRowsAtOnce = 32 / kPieces;
@@ -776,11 +788,11 @@ TOKB200_API int tokb200_shared_prefix_tcgen05_pieces(int n_rows, int n_tiles, in
 // As tokb200_shared_prefix_attention; `parts` holds n_rows * nh * tile_pieces * (HEAD_DIM + 2) floats where there are tiles.
 TOKB200_API int tokb200_shared_prefix_tcgen05(
     const void* q, const void* k_pool, const void* v_pool, void* out, const int* block_table, int table_stride, const int* row_req,
-    const int* pos, const int* shared, const int* members, const int* tiles, int n_tiles, int n_rows, int pool_rows, int nh, int nkv,
+    const int* pos, const int* shared, const int* members, int n_listed, const int* tiles, int n_tiles, int n_rows, int pool_rows, int nh, int nkv,
     int d, int page, float scale, const float* sink, float softcap, int tile_pieces, int own_pieces, float* parts,
     cudaStream_t stream) {
   if (n_rows <= 0) return TOKB200_OK;
-  if (d != HEAD_DIM || nh <= 0 || nkv <= 0 || nh % nkv || nh / nkv > OWN_MAX_GROUP || page <= 0 || page % 8 || pool_rows <= 0 || n_tiles < 0 ||
+  if (d != HEAD_DIM || nh <= 0 || nkv <= 0 || nh % nkv || nh / nkv > OWN_MAX_GROUP || page <= 0 || page % 8 || pool_rows <= 0 || n_tiles < 0 || n_listed < 0 ||
       n_tiles > 65535 || n_rows > 65535 || nkv > 65535 || table_stride <= 0 || (long long)table_stride * page > 0x7fffffffLL ||
       tile_pieces < 1 || tile_pieces > SP_MAX_PIECES || own_pieces < 1 || own_pieces > OWN_MAX_CLUSTER || (own_pieces & (own_pieces - 1)))
     return TOKB200_BAD_SIZE;
@@ -814,8 +826,8 @@ TOKB200_API int tokb200_shared_prefix_tcgen05(
     // strictly behind its predecessor, as attention_tcgen05.cu explains
     status = launch_ordered(false, softcap > 0.f ? shared_prefix_tcgen05_kernel<true> : shared_prefix_tcgen05_kernel<false>,
                             dim3(tile_pieces, nkv, n_tiles), dim3(SP_THREADS), (size_t)kFaSmem, stream, map_k, map_v, (const __nv_bfloat16*)q,
-                            (const __nv_bfloat16*)v_pool, block_table, table_stride, row_req, members, (const int4*)tiles, nh, nkv, page,
-                            run, pool_rows, tile_pieces, scale * 1.4426950408889634f, softcap > 0.f ? scale / softcap : 0.f,
+                            (const __nv_bfloat16*)v_pool, block_table, table_stride, row_req, members, n_listed, (const int4*)tiles, n_rows, nh,
+                            nkv, page, run, pool_rows, tile_pieces, scale * 1.4426950408889634f, softcap > 0.f ? scale / softcap : 0.f,
                             softcap > 0.f ? softcap / scale : 0.f, acc_parts, stat_parts);
     if (status != TOKB200_OK) return status;
   }

@@ -143,8 +143,10 @@ class scratch_scope:
 # loaded; the host reads the word (plain memory, no CUDA call) wherever it has just
 # synchronised with the device, and raises.
 _LIBRARY_NAMES = {1: "gemm_tcgen05", 2: "attention_tcgen05", 3: "ffn_small_m", 4: "linear_stream",
-                  5: "layer_small_m", 6: "gemm_f32_tcgen05", 7: "shared_prefix_tcgen05"}
-_REASONS = {1: "a wait on a shared-memory barrier ran out", 2: "a wait between blocks ran out"}
+                  5: "layer_small_m", 6: "gemm_f32_tcgen05", 7: "shared_prefix_tcgen05",
+                  8: "shared_prefix"}
+_REASONS = {1: "a wait on a shared-memory barrier ran out", 2: "a wait between blocks ran out",
+            3: "a tile has more members than it may, or some that are not in the list or not rows of the batch"}
 _error_word = None          # (ctypes int at the host address, device address)
 _registered = {}            # id(library handle) -> handle: libraries that know the word
 
@@ -614,7 +616,8 @@ def shared_prefix_attention(q, k_pool, v_pool, out, block_table, row_req, pos, s
     (int32) are rows of the batch, each in one tile at most (-1: none); `shared` (int32, one a row) repeats the tile's
     `keys`, 0 for a row of no tile.  The common keys are read through the block table of the tile's first live member.  A row
     then sees its own keys from `shared` up to its position, so `shared` is at most the position + 1; `cache.sharing.plan`
-    makes the three from block tables.  Rows of request -1 are left as they are.  `sink` and `softcap` as in the other
+    makes the three from block tables.  A tile of more members, or with some that are not rows, is found on the device only:
+    `raise_if_error` raises for it once the device is done.  Rows of request -1 are left as they are.  `sink` and `softcap` as in the other
     attention kernels; `block_table`, `row_req`, `pos` as theirs."""
     what, rows, dtype = "shared_prefix_attention", q.shape[0], q.dtype
     if dtype not in _DTYPE_TAG or k_pool.dtype != dtype or v_pool.dtype != dtype or out.dtype != dtype:
@@ -641,7 +644,7 @@ def shared_prefix_attention(q, k_pool, v_pool, out, block_table, row_req, pos, s
     sink_at, cap, stream = _sink(sink, nh).value or 0, float(softcap or 0.0), _stream().value or 0
     if rows == 0:
         return
-    n_tiles, width = tiles.shape[0], block_table.shape[1]
+    n_tiles, listed, width = tiles.shape[0], members.numel(), block_table.shape[1]
     reach = width * page
     # the parts are of this launch alone: captured graphs and streams share nothing
     if dtype == torch.bfloat16 and shared_prefix_tcgen05_supported(nh, nkv, d, page) and (q_at | k_at | v_at | out_at) % 16 == 0:
@@ -649,12 +652,12 @@ def shared_prefix_attention(q, k_pool, v_pool, out, block_table, row_req, pos, s
             n_tiles, shared_at = 0, 0
         launch, tile_pieces, own_pieces = _shared_prefix_plan(d, rows, n_tiles, nkv, reach)
         scratch = torch.empty(rows * nh * tile_pieces * (d + 2), dtype=torch.float32, device=q.device) if n_tiles else None
-        _check(launch(q_at, k_at, v_at, out_at, table_at, width, req_at, pos_at, shared_at, members_at, tiles_at, n_tiles, rows, slots,
+        _check(launch(q_at, k_at, v_at, out_at, table_at, width, req_at, pos_at, shared_at, members_at, listed, tiles_at, n_tiles, rows, slots,
                       nh, nkv, d, page, scale, sink_at, cap, tile_pieces, own_pieces, 0 if scratch is None else scratch.data_ptr(), stream), what)
         return
     launch, tile_pieces, own_pieces = _shared_prefix_plan(0, rows, n_tiles, nkv, reach)
     scratch = torch.empty(rows * nh * (tile_pieces + own_pieces) * (d + 2), dtype=torch.float32, device=q.device)
-    _check(launch(q_at, k_at, v_at, out_at, _tag(q), table_at, width, req_at, pos_at, shared_at, members_at, tiles_at, n_tiles,
+    _check(launch(q_at, k_at, v_at, out_at, _tag(q), table_at, width, req_at, pos_at, shared_at, members_at, listed, tiles_at, n_tiles,
                   shared_prefix_tile_members(nh, nkv), rows, nh, nkv, d, page, scale, sink_at, cap, tile_pieces, own_pieces,
                   scratch.data_ptr(), stream), what)
 
@@ -666,11 +669,11 @@ def _shared_prefix_plan(d: int, rows: int, n_tiles: int, nkv: int, reach: int):
     if d:
         lib = _load("shared_prefix_tcgen05.cu", defines=(f"HEAD_DIM={d}",))
         launch, plan = lib.tokb200_shared_prefix_tcgen05, lib.tokb200_shared_prefix_tcgen05_pieces
-        launch.argtypes = [at] * 5 + [n] + [at] * 5 + [n] * 7 + [f, at, f, n, n, at, at]
+        launch.argtypes = [at] * 5 + [n] + [at] * 4 + [n, at] + [n] * 7 + [f, at, f, n, n, at, at]
     else:
         lib = _lib("shared_prefix")
         launch, plan = lib.tokb200_shared_prefix_attention, lib.tokb200_shared_prefix_pieces
-        launch.argtypes = [at] * 4 + [n, at, n] + [at] * 5 + [n] * 7 + [f, at, f, n, n, at, at]
+        launch.argtypes = [at] * 4 + [n, at, n] + [at] * 4 + [n, at] + [n] * 7 + [f, at, f, n, n, at, at]
     tile_pieces, own_pieces = n(1), n(1)
     plan(_i(rows), _i(n_tiles), _i(nkv), _i(reach), ctypes.byref(tile_pieces), ctypes.byref(own_pieces))
     return launch, tile_pieces.value, own_pieces.value
