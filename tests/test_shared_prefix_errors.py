@@ -49,3 +49,16 @@ def test_tiles_that_are_none_raise(nh, nkv, d, dtype, monkeypatch):
             ops.raise_if_error()
     near(call(b), want, b)
     ops.raise_if_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("nh, nkv, d", [(14, 2, 64), (6, 1, 20)])
+def test_a_tile_may_list_more_places_than_the_batch_has_rows(nh, nkv, d, dtype, monkeypatch):
+    """Members that are none (-1) take places too: five rows at the end of 24."""
+    from test_shared_prefix import make, near, plain
+    monkeypatch.setattr(ops, "SHARED_PREFIX_LITTLE", 0)
+    b = make(nh, nkv, d, 16, [(5, 3)], 1, [9, 20], dtype)
+    members = [-1] * 19 + b["members"]
+    near(call(b, members, [[0, 24, 48, 0]]), plain(b, 0.125), b)
+    ops.raise_if_error()

@@ -276,7 +276,7 @@ static int sp_launch(const void* q, const void* k_pool, const void* v_pool, void
                      int tile_members, int n_rows, int nh, int nkv, int d, int page, float scale, const float* sink, float softcap,
                      int tile_pieces, int own_pieces, float* parts, cudaStream_t stream) {
   const int group = nh / nkv;
-  const int members_most = tile_members < n_rows ? tile_members : n_rows;
+  const int members_most = n_listed < 1 ? 1 : tile_members < n_listed ? tile_members : n_listed;
   const int tile_chunks = (members_most * group + SP_PAIRS - 1) / SP_PAIRS, row_chunks = (group + SP_PAIRS - 1) / SP_PAIRS;
   const long long units = (long long)n_tiles * tile_chunks + (long long)n_rows * row_chunks;
   if (nkv > 65535 || units > 65535) return TOKB200_BAD_SIZE;
