@@ -62,3 +62,22 @@ def test_a_tile_may_list_more_places_than_the_batch_has_rows(nh, nkv, d, dtype, 
     members = [-1] * 19 + b["members"]
     near(call(b, members, [[0, 24, 48, 0]]), plain(b, 0.125), b)
     ops.raise_if_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("scale, softcap", [(-0.3, None), (-0.3, 20.0), (0.0, None), (0.0, 20.0), (1e-38, 20.0)])
+def test_scales_of_any_sign(scale, softcap, d, dtype, monkeypatch):
+    """A factor that turns the order of the scores around, or makes them all alike."""
+    from test_shared_prefix import make, near, plain, run
+    monkeypatch.setattr(ops, "SHARED_PREFIX_LITTLE", 0)
+    b = make(12, 2, d, 16, [(20, 40)], 3, [90, 5], dtype)
+    b["q"] *= 6
+    got, want = run(b, scale, softcap), plain(b, scale, softcap)
+    assert torch.isfinite(got).all()
+    if dtype == torch.bfloat16:
+        near(got, want, b)
+    else:
+        # scores of up to 400, each off by 12 steps of 2^-24 of that; outputs move by as much of what they weigh
+        assert (got - want).norm() <= 400 * 12 * 2 ** -24 * 4 * max(want.norm(), 1.0)

@@ -647,7 +647,10 @@ def shared_prefix_attention(q, k_pool, v_pool, out, block_table, row_req, pos, s
     n_tiles, listed, width = tiles.shape[0], members.numel(), block_table.shape[1]
     reach = width * page
     # the parts are of this launch alone: captured graphs and streams share nothing
-    if dtype == torch.bfloat16 and shared_prefix_tcgen05_supported(nh, nkv, d, page) and (q_at | k_at | v_at | out_at) % 16 == 0:
+    # the tensor-core kernel looks for the largest product q.k, and squashes products by cap / scale: a factor that turns their
+    # order around, or makes that more than a number, is the general one's
+    if dtype == torch.bfloat16 and shared_prefix_tcgen05_supported(nh, nkv, d, page) and (q_at | k_at | v_at | out_at) % 16 == 0 and \
+            (scale >= 0 if softcap is None else cap < 3e38 * scale):
         if rows * reach * nkv * d * 4 <= SHARED_PREFIX_LITTLE and reach * d <= 300000:
             n_tiles, shared_at = 0, 0
         launch, tile_pieces, own_pieces = _shared_prefix_plan(d, rows, n_tiles, nkv, reach)
