@@ -108,12 +108,12 @@ class Engine:
         self.builder.reserve_capacity(16 * 8192 + tables)
 
     def _shared_notes(self):
-        """One annotation a group of keys that attention may read behind common beginnings."""
+        """One annotation a group of keys that some layer's attention reads behind common beginnings."""
         from ..parts.attention import PagedAttention, SharedBeginnings
         size, notes = torch.empty((), dtype=self.runtime.dtype).element_size(), []
         for g, layout in enumerate(self.cache.groups):
             readers = [self.model.blocks[call.layer].mixer for call, binding in zip(self.model.order, self.bindings) if binding.group == g]
-            readers = [m for m in readers if isinstance(m, PagedAttention) and ops.shared_prefix_supported(m.nh, m.nkv, m.d)]
+            readers = [m for m in readers if isinstance(m, PagedAttention) and m.reads_common_keys(self.runtime.dtype, self.cache.page_size)]
             if layout.keeps_all and readers:
                 notes.append(SharedBeginnings(g, self.cache.page_size, layout.planes * layout.kv_heads * layout.head_dim * size,
                                               min(ops.shared_prefix_tile_members(m.nh, m.nkv) for m in readers),

@@ -289,6 +289,12 @@ class PagedAttention:
         words, count = ctx.views.get(_BY_LENGTH.key, (None, 0))
         return (words[4:4 + count], words[:1]) if count == ctx.n_tokens else (None, None)      # a row a request
 
+    def reads_common_keys(self, dtype, page_size: int) -> bool:
+        """Whether steps of single tokens may read keys that several of their requests hold once for all of them
+        (`SharedBeginnings`): in 32 bits, and in bfloat16 where the tensor-core kernels take the sizes."""
+        return self.window is None and self.chunk is None and ops.shared_prefix_supported(self.nh, self.nkv, self.d) and \
+            (dtype == torch.float32 or ops.shared_prefix_tcgen05_supported(self.nh, self.nkv, self.d, page_size))
+
     def attend(self, q, out, ctx, group, cache):
         """Choose the kernel by precision and by the shape of the batch.  A group that keeps one
         row a token (`cache.v_pool` None) is read as keys and as values: the values are then the
@@ -297,9 +303,7 @@ class PagedAttention:
         v_pool = cache.v_pool if cache.v_pool is not None else cache.k_pool
         sink = self.sink
         common = ctx.views.get(f"shared_beginnings_{cache.group}")
-        if common is not None and common[1] > 0 and ctx.max_q_len == 1 and self.window is None and self.chunk is None and \
-                ops.shared_prefix_supported(self.nh, self.nkv, self.d) and \
-                (q.dtype == torch.float32 or ops.shared_prefix_tcgen05_supported(self.nh, self.nkv, self.d, group.page_size)):
+        if common is not None and common[1] > 0 and ctx.max_q_len == 1 and self.reads_common_keys(q.dtype, group.page_size):
             (tiles, shared, members), n_tiles = common
             ops.shared_prefix_attention(q, k_pool, v_pool, out, group.block_table, ctx.row_req, ctx.pos, shared[:ctx.n_tokens],
                                         members, tiles[:n_tiles], self.nh, self.nkv, self.d, group.page_size, self.scale, sink=sink,
