@@ -678,13 +678,9 @@ TOKB200_API int tokb200_decode_attention(
   config.blockDim = dim3(DEC_THREADS);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
-  static const int overlap = [] {
-    const char* v = getenv("TOKB200_PDL");
-    return (v && v[0] == '0') ? 0 : 1;
-  }();
   cudaLaunchAttribute attribute[2];
   attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute[0].val.programmaticStreamSerializationAllowed = overlap;
+  attribute[0].val.programmaticStreamSerializationAllowed = tokb200_early_starts();
   attribute[1].id = cudaLaunchAttributeClusterDimension;
   attribute[1].val.clusterDim.x = (unsigned)most;
   attribute[1].val.clusterDim.y = 1;

@@ -87,6 +87,35 @@ TOKB200_API int tokb200_error_word_alloc(int** host_pointer, int** device_pointe
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;"); }
 
+// Whether this library's kernels may start early.
+// TOKB200_PDL=0 in the environment launches every kernel strictly after its predecessor;
+// TOKB200_PDL_OFF=name[,name...] does so for the kernels of the libraries whose file names
+// contain one of the names (to find which early start a fault depends on)
+TOKB200_API int tokb200_early_starts() {
+  static const int allowed = [] {
+    const char* v = getenv("TOKB200_PDL");
+    if (v && v[0] == '0') return 0;
+    const char* off = getenv("TOKB200_PDL_OFF");
+    Dl_info here;
+    if (off && off[0] && dladdr((const void*)&tokb200_set_error_word, &here) && here.dli_fname) {
+      const char* at = off;
+      while (*at) {
+        const char* end = strchr(at, ',');
+        const size_t n = end ? (size_t)(end - at) : strlen(at);
+        char name[128];
+        if (n > 0 && n < sizeof(name)) {
+          memcpy(name, at, n);
+          name[n] = 0;
+          if (strstr(here.dli_fname, name)) return 0;
+        }
+        at = end ? end + 1 : at + n;
+      }
+    }
+    return 1;
+  }();
+  return allowed;
+}
+
 // `early`: whether this launch may start before its predecessor has completed (false: the
 // kernel still takes part in the chain, its own successor may start early, but it starts
 // strictly after its predecessor).
@@ -108,33 +137,9 @@ static inline int launch_ordered(bool early, void (*kernel)(KArgs...), dim3 grid
   config.blockDim = block;
   config.dynamicSmemBytes = smem;
   config.stream = stream;
-  // TOKB200_PDL=0 in the environment launches every kernel strictly after its predecessor;
-  // TOKB200_PDL_OFF=name[,name...] does so for the kernels of the libraries whose file names
-  // contain one of the names (to find which early start a fault depends on)
-  static const int overlap = [] {
-    const char* v = getenv("TOKB200_PDL");
-    if (v && v[0] == '0') return 0;
-    const char* off = getenv("TOKB200_PDL_OFF");
-    Dl_info here;
-    if (off && off[0] && dladdr((const void*)&tokb200_set_error_word, &here) && here.dli_fname) {
-      const char* at = off;
-      while (*at) {
-        const char* end = strchr(at, ',');
-        const size_t n = end ? (size_t)(end - at) : strlen(at);
-        char name[128];
-        if (n > 0 && n < sizeof(name)) {
-          memcpy(name, at, n);
-          name[n] = 0;
-          if (strstr(here.dli_fname, name)) return 0;
-        }
-        at = end ? end + 1 : at + n;
-      }
-    }
-    return 1;
-  }();
   cudaLaunchAttribute attribute[1];
   attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute[0].val.programmaticStreamSerializationAllowed = early ? overlap : 0;
+  attribute[0].val.programmaticStreamSerializationAllowed = early ? tokb200_early_starts() : 0;
   config.attrs = attribute;
   config.numAttrs = 1;
   cudaError_t err = cudaLaunchKernelEx(&config, kernel, static_cast<KArgs>(args)...);

@@ -1019,13 +1019,9 @@ static int launch_tc_persistent(const void* x, const void* w, const float* bias,
   config.blockDim = dim3(TC_THREADS);
   config.dynamicSmemBytes = (size_t)S::kTotal;
   config.stream = stream;
-  static const int overlap = [] {
-    const char* v = getenv("TOKB200_PDL");
-    return (v && v[0] == '0') ? 0 : 1;
-  }();
   cudaLaunchAttribute attribute[2];
   attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute[0].val.programmaticStreamSerializationAllowed = overlap;
+  attribute[0].val.programmaticStreamSerializationAllowed = tokb200_early_starts();
   attribute[1].id = cudaLaunchAttributeClusterDimension;
   attribute[1].val.clusterDim.x = 2;
   attribute[1].val.clusterDim.y = 1;

@@ -836,13 +836,9 @@ TOKB200_API int tokb200_shared_prefix_tcgen05(
   config.blockDim = dim3(OWN_THREADS);
   config.dynamicSmemBytes = own_smem;
   config.stream = stream;
-  static const int overlap = [] {
-    const char* v = getenv("TOKB200_PDL");
-    return (v && v[0] == '0') ? 0 : 1;
-  }();
   cudaLaunchAttribute attribute[2];
   attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute[0].val.programmaticStreamSerializationAllowed = overlap;
+  attribute[0].val.programmaticStreamSerializationAllowed = tokb200_early_starts();
   attribute[1].id = cudaLaunchAttributeClusterDimension;
   attribute[1].val.clusterDim.x = (unsigned)own_pieces;
   attribute[1].val.clusterDim.y = attribute[1].val.clusterDim.z = 1;
