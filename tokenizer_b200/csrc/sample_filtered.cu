@@ -786,7 +786,9 @@ sample_filtered_kernel(const float* __restrict__ logits, int vocab, int slice, i
 // rows are cut into 8 slices, many into 2.  Slices below some 3,000 logits are not worth an exchange.  us for 8 / 4 / 2 / 1
 // blocks, rows with settings of their own: 152,064 logits, 8 rows 39 / 53 / 89 / 151, 24 50 / 50 / 78 / 127, 64 103 / 91 / 124 / 206 (all
 // from a nucleus 134 / 98 / 82 / 131); 49,999, 8 rows 31 / 35 / 43 / 66, 37 56 / 48 / 58 / 88, 64 77 / 52 / 58 / 89 (from a nucleus 93 / 57 /
-// 38 / 56); 10,007, 37 rows 48 / 36 / 37 / 36; 2,000, 8 rows 20 / 19 / 19 / 18.
+// 38 / 56); 10,007, 37 rows 48 / 36 / 37 / 36; 2,000, 8 rows 20 / 19 / 19 / 18.  Which is faster goes by
+// the settings too, and those are on the device: the rule bears its loss where they are of the other kind (64 rows of 152,064 from a
+// nucleus 98 where 2 blocks take 82; of 49,999 with settings of their own 37 rows 58 where 4 take 48, 64 rows 58 where 4 take 52).
 static int fs_cluster(int n_rows, int vocab) {
   const int by_rows = n_rows <= 15 ? 8 : n_rows <= (vocab > 100000 ? 68 : 34) ? 4 : 2;
   const int by_slice = vocab > 24576 ? 8 : vocab > 8192 ? 4 : vocab > 3000 ? 2 : 1;

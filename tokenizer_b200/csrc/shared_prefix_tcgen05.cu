@@ -12,6 +12,11 @@
 //    own keys, the group's heads as one product (a warp takes 32 keys a turn; the next keys are asked for when the scores are
 //    computed, the next values when the weighted sum is); the pieces meet in distributed shared memory, and each block joins
 //    every size-th head with the parts of the first kernel.
+// Rounding: both kernels round a weight to bfloat16 in front of the second product, half a step (2^-8 of it at most), as the
+// framework's other attention on tensor cores does (a second product for what the rounding leaves would double that one's time);
+// sums of weights, weighted values and everything that is joined stay in 32 bits.  4 to 64 rows behind 512 to 8,192
+// keys are 0.0019 to 0.0023 off 64 bits (relative 2-norm), where the output's own rounding is 0.0017; the same inputs give the same bits.
+//
 // The first kernel lets the second start at once: what it reads but the parts (rows, tables, q, keys and values) was complete
 // before the first kernel began, which starts strictly behind its predecessor.  Its blocks take the multiprocessors that the
 // first kernel leaves and those that it has done with, and wait for it only in front of the join.
